@@ -39,6 +39,15 @@ struct Library {
   decltype(&::bsattn_bwd_tokens) bwd = nullptr;
   decltype(&::bsattn_reorder_inplace_workspace) reorder_workspace = nullptr;
   decltype(&::bsattn_reorder_inplace) reorder = nullptr;
+  decltype(&::bsattn_cache_append_workspace) cache_append_workspace = nullptr;
+  decltype(&::bsattn_cache_append) cache_append = nullptr;
+  decltype(&::bsattn_cache_read) cache_read = nullptr;
+  decltype(&::bsattn_cache_attn_workspace) cache_attn_workspace = nullptr;
+  decltype(&::bsattn_cache_attn) cache_attn = nullptr;
+  decltype(&::bsattn_cache_fork) cache_fork = nullptr;
+  decltype(&::bsattn_cache_free) cache_free = nullptr;
+  decltype(&::bsattn_cache_compact_workspace) cache_compact_workspace = nullptr;
+  decltype(&::bsattn_cache_compact) cache_compact = nullptr;
 } lib;
 
 void bind(const std::string& path) {
@@ -62,6 +71,15 @@ void bind(const std::string& path) {
   get(lib.bwd, "bsattn_bwd_tokens");
   get(lib.reorder_workspace, "bsattn_reorder_inplace_workspace");
   get(lib.reorder, "bsattn_reorder_inplace");
+  get(lib.cache_append_workspace, "bsattn_cache_append_workspace");
+  get(lib.cache_append, "bsattn_cache_append");
+  get(lib.cache_read, "bsattn_cache_read");
+  get(lib.cache_attn_workspace, "bsattn_cache_attn_workspace");
+  get(lib.cache_attn, "bsattn_cache_attn");
+  get(lib.cache_fork, "bsattn_cache_fork");
+  get(lib.cache_free, "bsattn_cache_free");
+  get(lib.cache_compact_workspace, "bsattn_cache_compact_workspace");
+  get(lib.cache_compact, "bsattn_cache_compact");
 }
 
 void check(int rc, const char* what) {
@@ -530,6 +548,207 @@ std::optional<int> reorder_inplace(const std::vector<Tensor>& tensors, const Ten
   return rc;
 }
 
+// ---- KV cache in pages, 4 bits ----
+// Where a cache's kernels say what they could not do: words of pinned host memory, never given back (a kernel may still be on its way
+// when its cache goes).
+int32_t* status_words() {
+  constexpr int64_t STEP = 16, CACHES = 256;
+  static std::mutex mu;
+  static Tensor* slab = nullptr;
+  static int64_t next = CACHES;
+  const std::lock_guard<std::mutex> lock(mu);
+  if (next == CACHES) {
+    slab = new Tensor(at::zeros({STEP * CACHES}, at::TensorOptions().dtype(at::kInt).pinned_memory(true)));
+    next = 0;
+  }
+  return slab->data_ptr<int32_t>() + STEP * next++;
+}
+
+struct PagedCache : torch::CustomClassHolder {
+  Tensor k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, free_from;
+  bsattn_cache c{};
+  int64_t head_dim;                 // of q, k, v (16 and 32 are kept as 64, with zeros behind them)
+  at::ScalarType dtype;
+
+  PagedCache(const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table, const Tensor& len, const Tensor& ref,
+             int64_t head_dim_, at::ScalarType dtype_)
+      : k_codes(kc), k_scales(ks), v_codes(vc), v_scales(vs), page_table(table), lengths(len), refs(ref), head_dim(head_dim_), dtype(dtype_) {
+    if (dtype != at::kHalf && dtype != at::kBFloat16) throw py::type_error("a cache is of float16 or bfloat16");
+    if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
+      throw py::value_error("head dimension must be 16, 32, 64, 128 or 256");
+    const int64_t D = std::max<int64_t>(head_dim, 64);
+    for (const Tensor* t : {&kc, &ks, &vc, &vs, &table, &len, &ref}) {
+      if (!t->is_cuda() || t->device() != kc.device()) throw std::runtime_error("a cache's tensors must all live on one GPU (there is no CPU path)");
+      if (!t->is_contiguous()) throw py::value_error("a cache's tensors must be contiguous");
+      if (t->scalar_type() != (t == &table || t == &len || t == &ref ? at::kInt : at::kByte))
+        throw py::type_error("a cache's codes and scales are uint8, page_table, lengths and refs int32");
+    }
+    if (kc.dim() != 4 || kc.size(2) != BSATTN_PAGE || kc.size(3) != D / 2 || vc.sizes() != kc.sizes())
+      throw py::value_error("codes must be [pages, heads, 64, head_dim / 2]");
+    const std::vector<int64_t> scales{kc.size(0), kc.size(1), D / 32, 4, 4, 4};
+    if (ks.sizes() != at::IntArrayRef(scales) || vs.sizes() != ks.sizes()) throw py::value_error("scales must be [pages, heads, head_dim / 32, 4, 4, 4]");
+    if (table.dim() != 2 || len.dim() != 1 || ref.dim() != 1 || table.size(0) != len.size(0) || ref.size(0) != kc.size(0))
+      throw py::value_error("page_table must be [sequences, pages of one], lengths [sequences], refs [pages]");
+    if (kc.numel() == 0 || table.numel() == 0) throw py::value_error("a cache has at least one page, head and sequence");
+    for (int64_t n : {kc.size(0), kc.size(1), table.size(0), table.size(1)})
+      if (n > INT_MAX) throw py::value_error("a cache's pages, heads and sequences are counted in 32 bits");
+    free_from = at::zeros({1}, ref.options());
+    c.k_codes = (uint8_t*)kc.data_ptr(); c.k_scales = (uint8_t*)ks.data_ptr();
+    c.v_codes = (uint8_t*)vc.data_ptr(); c.v_scales = (uint8_t*)vs.data_ptr();
+    c.page_table = table.data_ptr<int32_t>(); c.lengths = len.data_ptr<int32_t>(); c.refs = ref.data_ptr<int32_t>();
+    c.free_from = free_from.data_ptr<int32_t>();
+    c.pages = (int32_t)kc.size(0); c.heads = (int32_t)kc.size(1); c.head_dim = (int32_t)D;
+    c.sequences = (int32_t)table.size(0); c.max_pages = (int32_t)table.size(1);
+    c.dtype = dtype_code(dtype);
+    size_t bytes = 0;
+    check(lib.cache_compact_workspace(&c, &bytes), "PagedCache4");     // (what is left of the sizes)
+    c.status = status_words();
+  }
+  at::Device device() const { return k_codes.device(); }
+
+  // What calls so far have reported, once
+  void poll() {
+    int found = -1;
+    for (int i = 0; i < BSATTN_CACHE_STATUS_WORDS; ++i)
+      if (__atomic_load_n(c.status + i, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(c.status + i, 0, __ATOMIC_RELAXED) != 0 && found < 0) found = i;
+    if (found == BSATTN_CACHE_BAD_ROW)
+      throw std::runtime_error("an earlier call on this cache had a row that it refused: a sequence that does not exist or that the call names twice, a position, "
+                               "count or keep outside the sequence or its table, or a fork onto a sequence that holds tokens or is a parent");
+    if (found == BSATTN_CACHE_FULL) throw std::runtime_error("an earlier append to this cache found no free page: what it was to append is not there");
+    if (found == BSATTN_CACHE_BAD_PAGE) throw std::runtime_error("an earlier call on this cache met a page number in page_table that the cache does not have");
+  }
+};
+using CachePtr = c10::intrusive_ptr<PagedCache>;
+using Index = std::optional<Tensor>;
+
+// Numbers for the rows of a call, as the kernels take them
+Tensor row_numbers(const Index& t, const char* name, int64_t rows, const PagedCache& cache) {
+  if (!t) return Tensor();
+  if (!t->is_cuda() || t->device() != cache.device()) throw std::runtime_error(std::string(name) + " must live on the cache's GPU");
+  if (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong) throw py::type_error(std::string(name) + " must be int32 or int64");
+  if (t->dim() != 1 || t->size(0) != rows) throw py::value_error(std::string(name) + " must hold one number for each of the " + std::to_string(rows) + " rows");
+  Tensor x = *t;
+  if (x.scalar_type() == at::kLong) x = x.clamp(INT_MIN, INT_MAX).to(at::kInt);
+  return x.contiguous();
+}
+const int32_t* numbers(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
+
+void check_tokens(const Tensor& x, const char* name, const PagedCache& cache) {
+  if (!x.is_cuda() || x.device() != cache.device()) throw std::runtime_error(std::string(name) + " must live on the cache's GPU (there is no CPU path)");
+  if (x.scalar_type() != cache.dtype) throw py::type_error(std::string(name) + " must be of the cache's type");
+  if (x.dim() != 4 || x.size(3) != cache.head_dim) throw py::value_error(std::string(name) + " must be [B, H, N, " + std::to_string(cache.head_dim) + "]");
+  if (x.size(0) < 1) throw py::value_error(std::string(name) + " has no rows");
+  if (x.size(0) > INT_MAX || x.size(1) > INT_MAX || x.size(2) > INT_MAX) throw py::value_error(std::string(name) + ": sizes are counted in 32 bits");
+  if (at::GradMode::is_enabled() && x.requires_grad()) throw std::runtime_error(std::string(name) + " requires a gradient, and a cache has none: detach it or use torch.no_grad()");
+}
+void check_rows_of(const PagedCache& cache, int64_t rows, const Index& sequences) {
+  if (!sequences && rows > cache.c.sequences) throw py::value_error("more rows than the cache has sequences");
+}
+
+void cache_append(const CachePtr& cache, const Tensor& k_, const Tensor& v_, const Index& at_, const Index& counts_, const Index& sequences_) {
+  check_tokens(k_, "k", *cache);
+  check_tokens(v_, "v", *cache);
+  const int64_t B = k_.size(0), N = k_.size(2);
+  if (k_.sizes() != v_.sizes() || k_.size(1) != cache->c.heads) throw py::value_error("k, v must both be [B, " + std::to_string(cache->c.heads) + ", N, D]");
+  if (B > BSATTN_CACHE_ROWS_MAX) throw py::value_error("at most " + std::to_string(BSATTN_CACHE_ROWS_MAX) + " rows an append");
+  check_rows_of(*cache, B, sequences_);
+  if (N > (int64_t)cache->c.max_pages * BSATTN_PAGE) throw py::value_error("more tokens than a sequence of the cache may hold");
+  cache->poll();
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(cache->device());
+  const Tensor at = row_numbers(at_, "at", B, *cache), counts = row_numbers(counts_, "counts", B, *cache), sequences = row_numbers(sequences_, "sequences", B, *cache);
+  const Tensor k = prepared(padded(k_)), v = prepared(padded(v_));
+  size_t bytes = 0;
+  check(lib.cache_append_workspace(&cache->c, (int)B, (int)N, &bytes), "bsattn_cache_append_workspace");
+  const hipStream_t stream = stream_of(k);
+  const WorkspaceLock lock;
+  const Tensor ws = workspace_locked(bytes, k.device(), stream);
+  check(lib.cache_append(&cache->c, k.const_data_ptr(), v.const_data_ptr(), k.strides().data(), v.strides().data(), numbers(sequences), numbers(at),
+                         numbers(counts), (int)B, (int)N, ws.data_ptr(), bytes, stream), "bsattn_cache_append");
+}
+
+std::tuple<Tensor, Tensor> cache_read(const CachePtr& cache, int64_t tokens, const Index& start_, const Index& sequences_) {
+  cache->poll();
+  const int64_t B = sequences_ ? sequences_->numel() : (start_ ? start_->numel() : cache->c.sequences);
+  if (tokens < 1 || tokens > INT_MAX) throw py::value_error("tokens must be at least 1");
+  if (B < 1 || B > INT_MAX) throw py::value_error("no rows to read");
+  check_rows_of(*cache, B, sequences_);
+  c10::DeviceGuard guard(cache->device());
+  const Tensor start = row_numbers(start_, "start", B, *cache), sequences = row_numbers(sequences_, "sequences", B, *cache);
+  const auto options = at::TensorOptions().dtype(cache->dtype).device(cache->device());
+  const Tensor k = at::empty({B, cache->c.heads, tokens, cache->c.head_dim}, options), v = at::empty(k.sizes(), options);
+  check(lib.cache_read(&cache->c, k.data_ptr(), v.data_ptr(), k.strides().data(), v.strides().data(), numbers(sequences), numbers(start), (int)B, (int)tokens,
+                       stream_of(k)), "bsattn_cache_read");
+  return {unpadded(k, cache->head_dim), unpadded(v, cache->head_dim)};
+}
+
+py::object cache_attention(const CachePtr& cache, const Tensor& q_, const std::optional<Tensor>& mask, double sm_scale, const Index& counts_, const Index& sequences_,
+                           bool out_fp32, bool return_lse) {
+  check_tokens(q_, "q", *cache);
+  const int64_t B = q_.size(0), H = q_.size(1), N = q_.size(2);
+  if (H < 1 || H % cache->c.heads != 0) throw py::value_error("q's heads must be a multiple of the cache's");
+  if (N < 1) throw py::value_error("empty sequence");
+  check_rows_of(*cache, B, sequences_);
+  if (mask) {
+    if (mask->scalar_type() != at::kBool) throw py::type_error("mask must be a torch.bool tensor");
+    if (!mask->is_cuda() || mask->device() != cache->device()) throw std::runtime_error("mask must live on the cache's GPU");
+    if (mask->dim() != 4 || (mask->size(0) != 1 && mask->size(0) != B) || (mask->size(1) != 1 && mask->size(1) != cache->c.heads && mask->size(1) != H) ||
+        (mask->size(2) != 1 && mask->size(2) != (N + BSATTN_PAGE - 1) / BSATTN_PAGE) || mask->size(3) != cache->c.max_pages)
+      throw py::value_error("mask must be [1 or B, 1 or the cache's heads or q's, 1 or a row for each 64 queries, " + std::to_string(cache->c.max_pages) + " pages]");
+  }
+  cache->poll();
+  at::NoGradGuard no_grad;
+  c10::DeviceGuard guard(cache->device());
+  const Tensor counts = row_numbers(counts_, "counts", B, *cache), sequences = row_numbers(sequences_, "sequences", B, *cache);
+  const Tensor q = prepared(padded(q_));
+  const at::ScalarType out_dtype = result_type(q, out_fp32);
+  const Tensor o = like(q, out_dtype);
+  Tensor lse;
+  if (return_lse) lse = at::empty({B, H, N}, q.options().dtype(at::kFloat));
+  size_t bytes = 0;
+  check(lib.cache_attn_workspace(&cache->c, (int)B, (int)H, (int)N, &bytes), "bsattn_cache_attn_workspace");
+  const hipStream_t stream = stream_of(q);
+  {
+    const WorkspaceLock lock;
+    const Tensor ws = workspace_locked(bytes, q.device(), stream);
+    check(lib.cache_attn(&cache->c, q.const_data_ptr(), o.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
+                         mask ? (const uint8_t*)mask->const_data_ptr() : nullptr, mask ? mask->strides().data() : nullptr, mask ? (int)mask->size(0) : 1,
+                         mask ? (int)mask->size(1) : 1, mask ? (int)mask->size(2) : 1, numbers(sequences), numbers(counts), (int)B, (int)H, (int)N,
+                         dtype_code(out_dtype), (float)sm_scale, q.strides().data(), o.strides().data(), ws.data_ptr(), bytes, stream), "bsattn_cache_attn");
+  }
+  return results(o, lse, cache->head_dim, return_lse);
+}
+
+void cache_fork(const CachePtr& cache, const Tensor& parents_, const Tensor& children_) {
+  cache->poll();
+  if (parents_.numel() < 1) throw py::value_error("no sequences to fork");
+  if (parents_.numel() > cache->c.sequences) throw py::value_error("more children than the cache has sequences");
+  c10::DeviceGuard guard(cache->device());
+  const Tensor parents = row_numbers(parents_, "parents", parents_.numel(), *cache), children = row_numbers(children_, "children", parents_.numel(), *cache);
+  check(lib.cache_fork(&cache->c, numbers(parents), numbers(children), (int)parents.numel(), stream_of(parents)), "bsattn_cache_fork");
+}
+
+void cache_free(const CachePtr& cache, const Index& sequences_, const Index& keep_) {
+  cache->poll();
+  const int64_t n = sequences_ ? sequences_->numel() : (keep_ ? keep_->numel() : cache->c.sequences);
+  if (n < 1) throw py::value_error("no sequences to free");
+  if (n > cache->c.sequences) throw py::value_error("more rows than the cache has sequences");
+  c10::DeviceGuard guard(cache->device());
+  const Tensor sequences = row_numbers(sequences_, "sequences", n, *cache), keep = row_numbers(keep_, "keep", n, *cache);
+  check(lib.cache_free(&cache->c, numbers(sequences), numbers(keep), (int)n, stream_of(cache->lengths)), "bsattn_cache_free");
+}
+
+void cache_compact(const CachePtr& cache) {
+  cache->poll();
+  c10::DeviceGuard guard(cache->device());
+  size_t bytes = 0;
+  check(lib.cache_compact_workspace(&cache->c, &bytes), "bsattn_cache_compact_workspace");
+  const hipStream_t stream = stream_of(cache->lengths);
+  const WorkspaceLock lock;
+  const Tensor ws = workspace_locked(bytes, cache->device(), stream);
+  check(lib.cache_compact(&cache->c, ws.data_ptr(), bytes, stream), "bsattn_cache_compact");
+}
+
 std::optional<Tensor> defined_or_none(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 }  // namespace
@@ -552,6 +771,18 @@ PYBIND11_MODULE(_host, m) {
         py::arg("lists_t").none(true), py::arg("grid"), py::arg("sm_scale"), py::arg("out_fp32"), py::arg("return_lse"));
   m.def("set_python_lists", [](py::object make, py::object keep) { python_lists = new PythonLists{std::move(make), std::move(keep)}; });
   m.def("forward_backward", &forward_backward);
+  m.def("cache_append", &cache_append);
+  m.def("cache_read", &cache_read);
+  m.def("cache_attention", &cache_attention);
+  m.def("cache_fork", &cache_fork);
+  m.def("cache_free", &cache_free);
+  m.def("cache_compact", &cache_compact);
+  py::class_<PagedCache, CachePtr>(m, "PagedCache")
+      .def(py::init([](const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table, const Tensor& lengths, const Tensor& refs,
+                       int64_t head_dim, const Tensor& like) {
+        return c10::make_intrusive<PagedCache>(kc, ks, vc, vs, table, lengths, refs, head_dim, like.scalar_type());
+      }))
+      .def("poll", [](PagedCache& c) { c.poll(); });
   py::class_<TileLists, ListsPtr>(m, "TileLists")
       .def(py::init([](int64_t Bm, int64_t Hm, int64_t nb, py::object device, bool want_groups) {
              return c10::make_intrusive<TileLists>(Bm, Hm, nb, at::Device(py::cast<std::string>(py::str(device))), want_groups);

@@ -55,6 +55,15 @@ _SIGNATURES = {
     "bsattn_bwd_elementwise": ([_p] * 15 + [_i] * 8 + [_f] + [_p] * 8 + [_p, ctypes.c_size_t, _p], _i),
     "bsattn_reorder_inplace_workspace": ([_i] * 8 + [ctypes.POINTER(ctypes.c_size_t)], _i),
     "bsattn_reorder_inplace": ([_p, _p] + [_i] * 8 + [_p, _i, _i, _p, ctypes.c_size_t, _p], _i),
+    "bsattn_cache_append_workspace": ([_p, _i, _i, ctypes.POINTER(ctypes.c_size_t)], _i),
+    "bsattn_cache_append": ([_p] * 8 + [_i, _i, _p, ctypes.c_size_t, _p], _i),
+    "bsattn_cache_read": ([_p] * 7 + [_i, _i, _p], _i),
+    "bsattn_cache_attn_workspace": ([_p, _i, _i, _i, ctypes.POINTER(ctypes.c_size_t)], _i),
+    "bsattn_cache_attn": ([_p] * 6 + [_i] * 3 + [_p, _p] + [_i] * 4 + [_f, _p, _p, _p, ctypes.c_size_t, _p], _i),
+    "bsattn_cache_fork": ([_p, _p, _p, _i, _p], _i),
+    "bsattn_cache_free": ([_p, _p, _p, _i, _p], _i),
+    "bsattn_cache_compact_workspace": ([_p, ctypes.POINTER(ctypes.c_size_t)], _i),
+    "bsattn_cache_compact": ([_p, _p, ctypes.c_size_t, _p], _i),
     "bsattn_reorder": ([_p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p], _i),
 }
 EXPORTS = tuple(_SIGNATURES)

@@ -56,7 +56,7 @@ extern "C" {
  *   100: first layout.
  *   200: bsattn_bwd and bsattn_bwd_elementwise take dq_strides, dk_strides, dv_strides after
  *        do_strides; the entry points of the forward over quads of row blocks are gone. */
-#define BSATTN_ABI_VERSION 204
+#define BSATTN_ABI_VERSION 205
 int bsattn_version(void);
 /* Process-wide switch (default off), returns the previous setting.  On: the forward's result
  * depends on nothing but its inputs and the device (two runs give the same bits).  Off: the
@@ -371,6 +371,80 @@ int bsattn_reorder_inplace_workspace(int n, int BS, int NH, int F, int Hh, int W
 int bsattn_reorder_inplace(void* const* x, const int64_t* strides, int n, int BS, int NH, int F, int Hh, int W,
                            int D, int elem_bytes, const void* numbers, int number_bytes, int inverse,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * A KV cache held in 4 bits, in pages of 64 tokens (a page is the keys of one 64x64 tile), and the attention of new
+ * tokens over it.  No counterpart in the reference, whose one call takes the keys of a whole sequence in 16 bits
+ * (fa2_custom_mask/fa2_custom_mask.py:43-94); masks mean what they mean there: which 64-token blocks are kept.
+ *
+ * All of a cache's state is caller-owned device memory, so every call can be captured into a graph and replayed while
+ * the sequences grow; the library never reads it on the host.  A call that finds something it cannot do (a row that names
+ * no sequence, no free page) leaves that row as it was and writes 1 into a word of `status`.
+ *
+ * Values.  32 consecutive values of a token's head share a power of two: the smallest 2^e of which the largest magnitude
+ * is less than 7 times as large, e between -127 and 13 (fp16) or 125 (bf16); byte e + 127 is kept.  A value is the
+ * nearest of {0, .5, 1, 1.5, 2, 3, 4, 6} times that (of two equally near ones the one of even index), 6 times it at most,
+ * with its sign; code = index | sign << 3.  Values that are not finite make their 32 not a number (byte 255, codes 0).
+ * ---------------------------------------------------------------------------------- */
+#define BSATTN_PAGE 64
+#define BSATTN_CACHE_ROWS_MAX 1024 /* rows (sequences) of one append */
+/* words of bsattn_cache.status */
+#define BSATTN_CACHE_BAD_ROW 0  /* no such sequence, one that an earlier row of the call names too, a position or a count
+                                   outside the sequence or its table; fork: a child that holds tokens or is also a parent */
+#define BSATTN_CACHE_FULL 1     /* no free page for what a row appends */
+#define BSATTN_CACHE_BAD_PAGE 2 /* the page table names a page that the cache does not have */
+#define BSATTN_CACHE_STATUS_WORDS 3
+typedef struct {
+  uint8_t *k_codes, *v_codes;   /* [pages, heads, 64, head_dim / 2]: value 2 i in the lower four bits of byte i */
+  uint8_t *k_scales, *v_scales; /* [pages, heads, head_dim / 32, 4, 4, 4]: token t at [t % 4, t / 4 % 4, t / 16] */
+  int32_t* page_table;          /* [sequences, max_pages]: pages of a sequence in their order, -1 behind them */
+  int32_t* lengths;             /* [sequences] tokens */
+  int32_t* refs;                /* [pages] sequences that hold the page, 0: free */
+  int32_t* free_from;           /* 1 word: no page below this number is free (0 is always right) */
+  int32_t* status;              /* BSATTN_CACHE_STATUS_WORDS words, device or pinned host memory, or NULL */
+  int32_t pages, heads, head_dim, sequences, max_pages;
+  int32_t dtype;                /* BSATTN_F16 or BSATTN_BF16: of what is appended, read back and asked with */
+} bsattn_cache;
+
+/* In all calls: `sequences`, int32 [rows] in device memory, says which sequence of the cache a row of the call is (NULL: row
+ * b is sequence b).  All code and scale tensors are 16-byte aligned.
+ *
+ * Append: row b's sequence is cut to its first at[b] tokens (NULL: none are cut) and the first counts[b] (NULL: N) of the N tokens
+ * of k, v [B,heads,N,head_dim] go behind them.  Pages: those of the sequence that no other holds are written where they are; where
+ * there is none, or others hold it too, the free page of lowest number is taken, in the order of rows and tokens (of a page that
+ * others hold the tokens in front of at[b] are copied into it).  Pages behind the new end are given up.  A row for which there
+ * are no pages left is refused, rows behind it that need any too.  k, v: strides in elements of 4 dimensions, innermost 1, rows
+ * 16-byte aligned.  Pages given up in a call are free for the next one. */
+int bsattn_cache_append_workspace(const bsattn_cache* cache, int B, int N, size_t* bytes);
+int bsattn_cache_append(const bsattn_cache* cache, const void* k, const void* v, const int64_t* k_strides,
+                        const int64_t* v_strides, const int32_t* sequences, const int32_t* at, const int32_t* counts,
+                        int B, int N, void* workspace, size_t workspace_bytes, void* stream);
+/* The values of tokens start[b] .. start[b] + N - 1 (NULL: from 0) of each row's sequence into k, v [B,heads,N,head_dim] of the
+ * cache's type; zeros for tokens that the sequence does not have. */
+int bsattn_cache_read(const bsattn_cache* cache, void* k, void* v, const int64_t* k_strides, const int64_t* v_strides,
+                      const int32_t* sequences, const int32_t* start, int B, int N, void* stream);
+/* Attention of q [B,H,N,head_dim] over the cache, H a multiple of its heads (consecutive heads of q share one).  The first
+ * counts[b] (NULL: N) queries of row b are the last counts[b] tokens of its sequence: query i sits at position
+ * lengths - counts[b] + i and sees the tokens up to there.  mask: NULL, or bytes != 0 for the pages that are kept,
+ * [1|B, 1|heads|H, 1|ceil(N/64), max_pages], with element strides mask_strides; dimension 2: one row for all queries, or one for
+ * each 64 of the call.  o [B,H,N,head_dim] of out_dtype (the cache's or BSATTN_F32), lse fp32 [B,H,N] or NULL, as bsattn_fwd; queries
+ * that see no token, and those behind counts[b], get O = 0, lse = -inf. */
+int bsattn_cache_attn_workspace(const bsattn_cache* cache, int B, int H, int N, size_t* bytes);
+int bsattn_cache_attn(const bsattn_cache* cache, const void* q, void* o, float* lse, const uint8_t* mask,
+                      const int64_t* mask_strides, int Bm, int Hm, int Nm, const int32_t* sequences,
+                      const int32_t* counts, int B, int H, int N, int out_dtype, float sm_scale,
+                      const int64_t* q_strides, const int64_t* o_strides, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* children[i], which holds no tokens, becomes a copy of parents[i] that shares its pages (the next append to either copies the
+ * page that it writes to).  No sequence may be named twice in children, or in both. */
+int bsattn_cache_fork(const bsattn_cache* cache, const int32_t* parents, const int32_t* children, int n, void* stream);
+/* Sequences (NULL: the first n) keep their first keep[i] (NULL: 0) tokens and give up the pages behind them; a sequence that
+ * has no more than that stays as it is. */
+int bsattn_cache_free(const bsattn_cache* cache, const int32_t* sequences, const int32_t* keep, int n, void* stream);
+/* The pages in use get the lowest numbers: with U of them, the free page numbers below U, in ascending order, take the used pages
+ * from U on, in ascending order. */
+int bsattn_cache_compact_workspace(const bsattn_cache* cache, size_t* bytes);
+int bsattn_cache_compact(const bsattn_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
