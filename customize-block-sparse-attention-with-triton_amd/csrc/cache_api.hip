@@ -77,7 +77,9 @@ int bsattn_cache_attn_workspace(const bsattn_cache* cache, int B, int H, int N, 
   if (const int rc = check_cache(cache); rc != BSATTN_OK) return rc;
   if (bytes == nullptr) return BSATTN_ERR_NULL;
   if (B <= 0 || H <= 0 || N <= 0 || H % cache->heads != 0) return BSATTN_ERR_SHAPE;
-  if ((int64_t)N * (H / cache->heads) > 0x3fffffffLL || (int64_t)B * H * N > 0x7fffffffLL) return BSATTN_ERR_RANGE;
+  // rows of a tile are told apart with products of 32 bits
+  const int64_t group = H / cache->heads;
+  if (N * group > 0x3fffffffLL || N * group > 0xffffffffLL / group || (int64_t)B * H * N > 0x7fffffffLL) return BSATTN_ERR_RANGE;
   *bytes = cache_attn_workspace_bytes(*cache, B, H, N);
   return BSATTN_OK;
 }

@@ -14,12 +14,21 @@
 // conversions, 64 byte permutes for V and about 200 other vector instructions against 8.7 KB, 32 matrix instructions per 16 rows.
 // Prompt pieces have 64 rows per tile: the conversions are shared by four times as many products and the matrix cores bound it.
 //
-// Who walks what.  The pages of a (sequence, tile) are dealt round robin to `splits` x 4 wavefronts (so that a mask's dense stretches, the
-// last blocks for instance, go to all of them); splits in proportion to the pages, found on the device from the lengths: the host never
-// knows them, and a captured launch follows sequences as they grow.  The four wavefronts of a workgroup meet in LDS, workgroups in the
-// workspace: the last one in adds up all parts in their order (count_in in fwd_tile.h), so results do not depend on the pace.
+// Who walks what.  The pages of all (sequence, tile) units of a head lie behind each other on an axis that is cut into equal ranges, one for
+// each workgroup that the GPU holds at a time (a unit's end counts GAP pages: a workgroup that goes on into the next one has a merge to
+// do; a cut next to a unit's begin or end goes there).  Where the cuts fall the device finds out from the lengths: the host never knows
+// them, and a captured launch follows sequences as they grow.  A range's pages go round robin to the workgroup's four wavefronts, which meet in
+// LDS.  With a mask the pages of a unit lie on the axis in columns of STEP (one of each 1 / STEP of the sequence): what a mask keeps next to
+// each other, the last blocks for instance, goes to all of the unit's workgroups.
+//
+// Units of several workgroups meet in the workspace, without a counter (64 workgroups that count themselves in by compare-and-swap took
+// 200 us).  Each stores its part, waits until the stores are acknowledged, stores the launch's mark into its flag, waits for that, and
+// reads the flags of all: the last one to store its flag sees them all set, and adds up the parts in their order.  More than one may
+// see that; they write the same bits.  Nobody waits for anybody.  Who sees all flags clears them, so that a replay of a captured launch,
+// which carries the same mark, finds none set; what other launches have left carries another mark.
 #include <hip/hip_runtime.h>
 #include <algorithm>
+#include <cfloat>
 #include "common.h"
 #include "kernel_util.h"
 #include "cache.h"
@@ -27,6 +36,12 @@
 namespace bsattn {
 
 constexpr int WAVES = 4;
+constexpr int STEP = 16;                      // (see above)
+// Pages of the shortest range, and how near to a unit's end a cut goes there; a tile of more rows takes as much longer for a page.
+// (Fewer than GAP positions are never between two cuts, so that one cut at most is near an end.)
+template <int QT> constexpr int LEAST = QT == 1 ? 8 : 4;
+template <int QT> constexpr int NEAR = QT == 1 ? 6 : 3;
+template <int QT> constexpr int GAP = NEAR<QT> + 1;
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 // Numerators are 2^HEADROOM at most: in fp16, whose steps are equal below 2^-14, small ones keep their digits 15 powers of two further
 // down (without it weights of 2^-16 beside one of 1 were 2^-9 off).
@@ -36,21 +51,39 @@ constexpr float NO_MASS = -3.0e38f;           // reference exponent of a row tha
 struct CacheAttnParams {
   bsattn_cache c;
   CacheAttn a;
-  int group, rows, tiles, W, min_pages, max_splits;      // query heads per head of the cache; N * group; tiles of them; workgroups to share (0: a unit each)
+  int group, rows, tiles, W;      // query heads per head of the cache; N * group; tiles of them; workgroups of a head (0: one a unit)
+  unsigned per_group;             // 2^32 / group rounded up (by_group)
   float scale; unsigned flip;                            // |sm_scale| log2 e; sign bits if sm_scale < 0
   float *part_o, *part_ml;
-  unsigned long long *arrivals, epoch;
+  unsigned long long *flags, mark;
 };
 
-// Counts a part in, by one thread, once all accesses of its workgroup to it have been acknowledged; returns how many are in.  The counter
-// holds (launch mark << 16 | parts); stale contents carry another mark.
-__device__ __forceinline__ int count_part(unsigned long long* arrivals, unsigned long long epoch) {
-  unsigned long long seen = __hip_atomic_load(arrivals, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (;;) {     // (ends: the counter only changes when another part is counted, at most as often as there are parts)
-    const unsigned long long want = (seen >> 16) == epoch ? seen + 1 : ((epoch << 16) | 1ull);
-    if (__hip_atomic_compare_exchange_strong(arrivals, &seen, want, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-      return (int)(want & 0xffffull);
-  }
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+// Eight bytes that other workgroups have written (see coherent_load)
+__device__ __forceinline__ floatx2 coherent_load2(const float* p) {
+  return __builtin_bit_cast(floatx2, __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// row / group, exact for row * group < 2^32
+__device__ __forceinline__ int by_group(unsigned row, int group, unsigned per_group) { return group == 1 ? (int)row : (int)__umulhi(row, per_group); }
+
+// The kernel's arguments, from memory
+typedef const CacheAttnParams __attribute__((address_space(4)))* ParamsAgain;
+__device__ __forceinline__ ParamsAgain params_again() {
+  ParamsAgain p = (ParamsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+// Sum over the lanes up to this one
+__device__ __forceinline__ int wave_upto(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);       // lanes 1, 2, 4, 8 further down in a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);       // a row's last lane to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);       // lane 31 to the upper rows
+  return x;
 }
 
 template <bool BF16>
@@ -104,37 +137,40 @@ template <> struct Words<2> { typedef uintx2 type; };
 template <> struct Words<4> { typedef uintx4 type; };
 
 template <int D>
-__device__ __forceinline__ void load_page(PageRegs<D>& r, const bsattn_cache& c, int64_t at, int n, int g) {
+__device__ __forceinline__ void load_keys(PageRegs<D>& r, const bsattn_cache& c, int64_t at, int n, int g) {
   constexpr int ROW = D / 2;
-  const int krow = 4 * (n & 3) + (n >> 2);
-  const uint8_t* kc = c.k_codes + at * page_codes(D) + krow * ROW + g * (D / 8);
-  const uint8_t* ks = c.k_scales + at * page_scales(D) + (D == 64 ? g >> 1 : (D == 128 ? g : 2 * g)) * PAGE + n * 4;
-  const uint8_t* vc = c.v_codes + at * page_codes(D) + g * ROW + n * (D / 32);
-  const uint8_t* vs = c.v_scales + at * page_scales(D) + (D == 64 ? n >> 3 : (D == 128 ? n >> 2 : n >> 1)) * PAGE + g * 16;
+  const uint8_t* codes = c.k_codes + at * page_codes(D);
+  const uint8_t* scales = c.k_scales + at * page_scales(D);
+  const unsigned lane_codes = (4 * (n & 3) + (n >> 2)) * ROW + g * (D / 8);
+  const unsigned lane_scales = (D == 64 ? g >> 1 : (D == 128 ? g : 2 * g)) * PAGE + n * 4;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    if constexpr (D == 256) {
-      const uintx4 a = *reinterpret_cast<const uintx4*>(kc + t * 16 * ROW), b = *reinterpret_cast<const uintx4*>(kc + t * 16 * ROW + 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { r.k[t][i] = a[i]; r.k[t][4 + i] = b[i]; }
-    } else {
-      const auto a = *reinterpret_cast<const typename Words<D / 32>::type*>(kc + t * 16 * ROW);
+    for (int x = 0; x < D / 32; x += 4) {
+      const auto a = *reinterpret_cast<const typename Words<(D / 32 < 4 ? D / 32 : 4)>::type*>(codes + lane_codes + t * 16 * ROW + 4 * x);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) r.k[t][i] = a[i];
+      for (int i = 0; i < (D / 32 < 4 ? D / 32 : 4); ++i) r.k[t][x + i] = a[i];
     }
   }
 #pragma unroll
-  for (int i = 0; i < PageRegs<D>::KS; ++i) r.ks[i] = *reinterpret_cast<const unsigned*>(ks + i * PAGE);
+  for (int i = 0; i < PageRegs<D>::KS; ++i) r.ks[i] = *reinterpret_cast<const unsigned*>(scales + lane_scales + i * PAGE);
+}
+template <int D>
+__device__ __forceinline__ void load_values(PageRegs<D>& r, const bsattn_cache& c, int64_t at, int n, int g) {
+  constexpr int ROW = D / 2;
+  const uint8_t* codes = c.v_codes + at * page_codes(D);
+  const uint8_t* scales = c.v_scales + at * page_scales(D);
+  const unsigned lane_codes = g * ROW + n * (D / 32), lane_scales = (D == 64 ? n >> 3 : (D == 128 ? n >> 2 : n >> 1)) * PAGE + g * 16;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {              // token 16 (j / 4) + 4 (j % 4) + g
-    if constexpr (D == 64) r.v[j][0] = *reinterpret_cast<const unsigned short*>(vc + 4 * j * ROW);
-    else if constexpr (D == 128) r.v[j][0] = *reinterpret_cast<const unsigned*>(vc + 4 * j * ROW);
+    if constexpr (D == 64) r.v[j][0] = *reinterpret_cast<const unsigned short*>(codes + lane_codes + 4 * j * ROW);
+    else if constexpr (D == 128) r.v[j][0] = *reinterpret_cast<const unsigned*>(codes + lane_codes + 4 * j * ROW);
     else {
-      const uintx2 a = *reinterpret_cast<const uintx2*>(vc + 4 * j * ROW);
+      const uintx2 a = *reinterpret_cast<const uintx2*>(codes + lane_codes + 4 * j * ROW);
       r.v[j][0] = a[0]; r.v[j][1] = a[1];
     }
   }
-  r.vs = *reinterpret_cast<const uintx4*>(vs);
+  r.vs = *reinterpret_cast<const uintx4*>(scales + lane_scales);
 }
 
 // What tile `tile` of row b walks: its sequence, the position of the row's first query, and pages 0 .. pages - 1
@@ -149,149 +185,174 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& prm, int b, int t
     return u;
   }
   u.first = length_of(prm.c, u.seq) - u.count;
-  const int t0 = tile * ROWS / prm.group, t1 = (min(prm.rows, (tile + 1) * ROWS) - 1) / prm.group;
+  const int t0 = by_group(tile * ROWS, prm.group, prm.per_group), t1 = by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group);
   const int last = u.first + min(u.count - 1, t1);
   u.pages = t0 < u.count && last >= 0 ? last / PAGE + 1 : 0;
   return u;
 }
 
-template <int D, bool BF16, int QT>
-__global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) void cache_attn_kernel(const CacheAttnParams prm) {
+template <int D, bool BF16, int QT, bool MASK>
+__global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT == 1 && D <= 128 ? 3 : 2)) void cache_attn_kernel(const CacheAttnParams prm) {
   constexpr int ROWS = 16 * QT, PITCH = D + 4, KSTEPS = D / 32, DT = D / 16;
   extern __shared__ __align__(16) float lds[];           // [WAVES][ROWS][PITCH] parts of O | [WAVES][ROWS][2] (m, l) | [ROWS][2]
   float* const lds_ml = lds + WAVES * ROWS * PITCH;
   float* const lds_row = lds_ml + WAVES * ROWS * 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const bsattn_cache& c = prm.c;
-  const int h = blockIdx.x % (unsigned)c.heads;
+  const int h = blockIdx.x % (unsigned)c.heads, w = blockIdx.x / (unsigned)c.heads;
   const int units = prm.a.B * prm.tiles;
-  int unit = blockIdx.x / (unsigned)c.heads, split = 0, splits = 1, first_wg = 0;
-  // unit -> (row of the call, tile): the tiles with the most pages first
-  auto row_of = [&](int u) { return u % prm.a.B; };
-  auto tile_of = [&](int u) { return prm.tiles - 1 - u / prm.a.B; };
-  if (prm.W > 0) {
-    // the workgroups of a head, W + units of them, are given to the units in proportion to their pages (every wavefront finds out
-    // by itself)
-    const int w = unit;
-    int64_t total = 0;
-    for (int u0 = 0; u0 < units; u0 += 64) {
-      int p = 0;
-      if (u0 + lane < units) p = unit_of<ROWS>(prm, row_of(u0 + lane), tile_of(u0 + lane)).pages;
-      for (int x = 32; x > 0; x >>= 1) p += __shfl_xor(p, x);
-      total += p;
-    }
-    const int per = (int)max((int64_t)prm.min_pages, (total + prm.W - 1) / prm.W);
-    int before = 0;
-    unit = -1;
-    for (int u0 = 0; u0 < units && unit < 0; u0 += 64) {
-      int s = 0, pages = 0;
-      if (u0 + lane < units) {
-        pages = unit_of<ROWS>(prm, row_of(u0 + lane), tile_of(u0 + lane)).pages;
-        s = min(prm.max_splits, max(1, (pages + per - 1) / per));
-      }
-      int upto = s;
-      for (int x = 1; x < 64; x <<= 1) {
-        const int y = __shfl_up(upto, x);
-        if (lane >= x) upto += y;
-      }
-      const unsigned long long has = __ballot(before + upto > w);
-      if (has != 0) {
-        const int at = __builtin_ctzll(has);
-        unit = u0 + at;
-        splits = __builtin_amdgcn_readlane(s, at);
-        first_wg = before + __builtin_amdgcn_readlane(upto, at) - splits;
-        split = w - first_wg;
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (unit < 0) return;                     // (all wavefronts alike)
+  // positions of a unit's pages on the axis
+  auto positions = [&](int pages) { return MASK ? (pages + STEP - 1) / STEP * STEP : pages; };
+
+  // ---- the range ----
+  Unit mine = {-1, 0, 0, 0};                  // a lane's unit of 64, where it begins on the axis, and how much of the axis it has
+  int begin = 0, length = 0, behind = 0, lo = 0, hi = 0, total = 0, each = 1, longer = 0;
+  bool cut = false;                           // is the range known
+  auto cut_at = [&](int x) { return each * x + min(x, longer); };            // begin of range x
+  // the range that holds a position
+  auto holder = [&](int x) {
+    const int of_longer = (each + 1) * longer;
+    return x < of_longer ? (int)((unsigned)x / (unsigned)(each + 1)) : longer + (int)((unsigned)(x - of_longer) / (unsigned)each);
+  };
+
+  for (int base = prm.W > 0 ? 0 : w;;) {      // units base .. base + 63
+  length = 0;
+  const int lane_unit = base + lane;
+  if (prm.W > 0 ? lane_unit < units : lane == 0) {
+    mine = unit_of<ROWS>(prm, lane_unit % prm.a.B, prm.tiles - 1 - lane_unit / prm.a.B);
+    length = positions(mine.pages) + GAP<QT>;
   }
-  const int b = row_of(unit), tile = tile_of(unit);
-  const Unit un = unit_of<ROWS>(prm, b, tile);
-  const int pages = __builtin_amdgcn_readfirstlane(un.pages), stride = splits * WAVES, slot = split * WAVES + wave;
+  const int upto = wave_upto(length);
+  begin = behind + upto - length;
+  behind += __builtin_amdgcn_readlane(upto, 63);
+  if (!cut) {
+    if (prm.W > 0 && base + 64 < units) { base += 64; continue; }
+    total = behind;
+    hi = total;
+    if (prm.W > 0) {
+      const int ranges = min(prm.W, max(units, total / LEAST<QT>));
+      if (w >= ranges) return;
+      // the first `longer` ranges are one position longer than `each`
+      each = (unsigned)total / (unsigned)ranges; longer = total - each * ranges;
+      lo = each * w + min(w, longer);
+      hi = lo + each + (w < longer ? 1 : 0);
+    }
+    cut = true;
+    if (base > 0 && prm.W > 0) { base = 0; behind = 0; continue; }
+  }
+  for (unsigned long long mates = __ballot(length > 0 && begin < hi && begin + length > lo); mates != 0; mates &= mates - 1) {
+  const int at = __builtin_ctzll(mates), unit = base + at, b = unit % prm.a.B, tile = prm.tiles - 1 - unit / prm.a.B;
+  const Unit un = {__builtin_amdgcn_readlane(mine.seq, at), __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.count, at),
+                   __builtin_amdgcn_readlane(mine.pages, at)};
+  const int unit_begin = __builtin_amdgcn_readlane(begin, at), unit_positions = positions(un.pages);
+  int first_wg = w, last_wg = w;              // workgroups of the unit
+  if (prm.W > 0) {
+    first_wg = holder(unit_begin);
+    last_wg = unit_positions > 0 ? holder(unit_begin + unit_positions - 1) : first_wg;
+    if (first_wg < last_wg && cut_at(first_wg + 1) - unit_begin <= NEAR<QT>) ++first_wg;
+    if (first_wg < last_wg && unit_begin + unit_positions - cut_at(last_wg) <= NEAR<QT>) --last_wg;
+    if (w < first_wg || w > last_wg) continue;
+  }
+  const int splits = last_wg - first_wg + 1, split = w - first_wg;
+  const int from = split == 0 ? 0 : cut_at(w) - unit_begin, to = w == last_wg ? unit_positions : cut_at(w + 1) - unit_begin;      // its positions
 
   // ---- queries: B operands, lane (n, g) has columns g D / 4 + 8 s .. + 7 of row n ----
   uintx4 qf[QT][KSTEPS];
   int limit[QT];                              // last token that the lane's query sees
   const uint8_t* mrow[QT];                    // its row of the mask
-  const int block0 = prm.a.ms[2] != 0 ? (int)(tile * ROWS / prm.group) / PAGE : 0;        // rows of the mask that the tile's queries have
-  const int block1 = prm.a.ms[2] != 0 ? min((min(prm.rows, (tile + 1) * ROWS) - 1) / prm.group, max(un.count - 1, 0)) / PAGE : 0;
-  const bool rows_differ = prm.a.mask != nullptr && (prm.a.mask_heads == 2 || block0 < block1);
+  const bool by_head = MASK && prm.a.mask_heads == 2;
+  int block0 = 0, block1 = 0;                 // rows of the mask that the tile's queries have
+  const uint8_t* tile_mask = nullptr;         // the first of them, of the tile's first head
+  if constexpr (MASK) {
+    if (prm.a.ms[2] != 0) {
+      block0 = by_group(tile * ROWS, prm.group, prm.per_group) / PAGE;
+      block1 = max(block0, min(by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group), un.count - 1) / PAGE);
+    }
+    tile_mask = prm.a.mask + b * prm.a.ms[0] + (by_head ? h * prm.group : (prm.a.mask_heads == 1 ? h : 0)) * prm.a.ms[1] + block0 * prm.a.ms[2];
+  }
+  const bool rows_differ = MASK && (by_head || block0 < block1);
+  // last token that any of the tile's queries sees
+  const int last_token = un.first + min(un.count - 1, by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group));
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int r = tile * ROWS + 16 * qt + n;
-    const int token = r / prm.group, head = h * prm.group + (r - token * prm.group);
-    const bool real = r < prm.rows && token < un.count;
-    limit[qt] = real ? un.first + token : 0x7fffffff;       // (rows that are not asked for: their results are not written)
-    mrow[qt] = prm.a.mask;
-    if (rows_differ && real)
-      mrow[qt] += b * prm.a.ms[0] + (prm.a.mask_heads == 2 ? head : (prm.a.mask_heads == 1 ? h : 0)) * prm.a.ms[1] + (token / PAGE) * prm.a.ms[2];
-    else if (prm.a.mask != nullptr)
-      mrow[qt] += b * prm.a.ms[0] + (prm.a.mask_heads == 2 ? h * prm.group : (prm.a.mask_heads == 1 ? h : 0)) * prm.a.ms[1] +
-                  block0 * prm.a.ms[2];
+    const bool asked = r < prm.rows && by_group(r, prm.group, prm.per_group) < un.count;
+    const int row = asked ? r : tile * ROWS;                // (rows that are not asked for: any query will do, their results are not written)
+    const int token = by_group(row, prm.group, prm.per_group), of_group = row - token * prm.group;
+    limit[qt] = asked ? un.first + token : 0x7fffffff;
+    mrow[qt] = tile_mask;
+    if (rows_differ) mrow[qt] += (by_head ? of_group : 0) * prm.a.ms[1] + (block1 > block0 ? token / PAGE - block0 : 0) * prm.a.ms[2];
+    const unsigned short* q = (const unsigned short*)prm.a.q + b * prm.a.qs[0] + (h * prm.group + of_group) * prm.a.qs[1] + token * prm.a.qs[2] + g * (D / 4);
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      qf[qt][s] = uintx4{0, 0, 0, 0};
-      if (real) {
-        qf[qt][s] = *reinterpret_cast<const uintx4*>((const unsigned short*)prm.a.q + b * prm.a.qs[0] + head * prm.a.qs[1] + token * prm.a.qs[2] + g * (D / 4) + 8 * s);
+    for (int s = 0; s < KSTEPS; ++s) qf[qt][s] = *reinterpret_cast<const uintx4*>(q + 8 * s);
+  }
+  if (prm.flip != 0)
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) qf[qt][s][i] ^= prm.flip;
-      }
-    }
-  }
 
   floatx4 o[QT][DT];
   float m[QT], l[QT];
-  bool seen[QT];
+  unsigned marks = 0;                         // bit 4 qt + i: columns (4 g + i) DT .. are not numbers; bit 16 + qt: the query has seen a token
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    m[qt] = -INFINITY; l[qt] = 0.f; seen[qt] = false;
+    m[qt] = -INFINITY; l[qt] = 0.f;
 #pragma unroll
     for (int s = 0; s < DT; ++s) o[qt][s] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- the wavefront's pages: slot + i * stride, 64 of them looked up at a time ----
-  const int mine = pages > slot ? (pages - slot + stride - 1) / stride : 0;
+  // ---- the wavefront's positions: from + wave + 4 i, 64 of them looked up at a time ----
+  const int own = to > from + wave ? (to - from - wave + WAVES - 1) / WAVES : 0, columns = unit_positions / STEP;
   int chunk = -64, table = -1;
   unsigned long long bits = 0;
-  const int heads_kept = prm.a.mask_heads == 2 ? prm.group : 1;
+  auto page_at = [&](int i) {                 // page of the wavefront's position i
+    const int x = from + wave + WAVES * i;
+    return MASK ? (x % STEP) * columns + x / STEP : x;
+  };
   // next kept page: its number in the cache and in the sequence
   auto next = [&](int& page, int& index) -> bool {
     while (bits == 0) {
       chunk += 64;
-      if (chunk >= mine) return false;
-      const int i = chunk + lane, p = slot + i * stride;
-      bool keep = i < mine;
+      if (chunk >= own) return false;
+      const int p = page_at(chunk + lane);
+      const bool there = chunk + lane < own && p < un.pages;
       table = -1;
-      if (keep) {
-        table = c.page_table[(int64_t)un.seq * c.max_pages + p];
-        if (table < 0 || table >= c.pages) { report(c.status, STATUS_PAGE); keep = false; }
-      }
-      if (prm.a.mask != nullptr && keep) {
-        // kept by any of the tile's queries
-        const uint8_t* row = prm.a.mask + b * prm.a.ms[0] + (prm.a.mask_heads == 2 ? h * prm.group : (prm.a.mask_heads == 1 ? h : 0)) * prm.a.ms[1] + p * prm.a.ms[3];
-        keep = false;
-        for (int q = block0; q <= block1; ++q)
-          for (int x = 0; x < heads_kept; ++x) keep |= row[x * prm.a.ms[1] + q * prm.a.ms[2]] != 0;
-      }
+      bool keep = there && !MASK;
+      if (there) table = c.page_table[(int64_t)un.seq * c.max_pages + p];
+      if constexpr (MASK)                     // kept by any of the tile's queries
+        if (there)
+          for (int q = 0; q <= block1 - block0; ++q)
+            for (int x = 0; x < (by_head ? prm.group : 1); ++x) keep |= tile_mask[x * prm.a.ms[1] + q * prm.a.ms[2] + p * prm.a.ms[3]] != 0;
+      if (keep && (table < 0 || table >= c.pages)) { report(c.status, STATUS_PAGE); keep = false; }
       bits = __ballot(keep);
     }
     const int j = __builtin_ctzll(bits);
     bits &= bits - 1;
     page = __builtin_amdgcn_readlane(table, j);
-    index = slot + (chunk + j) * stride;
+    index = page_at(chunk + j);
     return true;
   };
-  auto load = [&](PageRegs<D>& r, int page, int index) {
-    load_page<D>(r, c, page_of_head(c, page, h), n, g);
-    if (rows_differ) {
+  // One page at a time.  Its keys' registers are free for the next page's once the scores are there, its values' once they are in O: the
+  // loads of a page are under way for most of the time that the page in front of it takes.
+  PageRegs<D> r = {};                         // (not left open: the compiler would keep a unit's last page for the next one)
+  int page = 0, index = 0;
+  auto load_kept = [&] {
+    if constexpr (MASK)
+      if (rows_differ)
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) r.kept[qt] = mrow[qt][index * prm.a.ms[3]];
-    }
+        for (int qt = 0; qt < QT; ++qt) r.kept[qt] = mrow[qt][index * prm.a.ms[3]];
   };
-
-  auto take = [&](const PageRegs<D>& r, int page, int index) {
-    const int base = index * PAGE;
+  bool more = next(page, index);
+  if (more) {
+    load_keys<D>(r, c, page_of_head(c, page, h), n, g);
+    load_values<D>(r, c, page_of_head(c, page, h), n, g);
+    load_kept();
+  }
+  while (more) {
+    const int token0 = index * PAGE, this_page = page;
     floatx4 s[QT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -309,35 +370,40 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) voi
     int see[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      see[qt] = rows_differ && limit[qt] != 0x7fffffff && r.kept[qt] == 0 ? -1 : limit[qt];
-      lacks |= see[qt] < base + PAGE - 1;
+      see[qt] = limit[qt];
+      if constexpr (MASK) if (rows_differ && limit[qt] != 0x7fffffff && r.kept[qt] == 0) see[qt] = -1;
+      lacks |= see[qt] < token0 + PAGE - 1;
     }
     const bool part = __ballot(lacks) != 0;
-    uintx4 vs = r.vs;
+    more = next(page, index);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) {
+      load_keys<D>(r, c, page_of_head(c, page, h), n, g);
+      load_kept();
+    }
     bool odd = false;                         // values that are not numbers in a page that not all queries see
     if (part) {
-      int last = -1;                          // last token that any query sees
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        if (see[qt] != 0x7fffffff) last = max(last, see[qt]);
+        const int up_to = see[qt] - token0 - g;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (base + 16 * t + 4 * i + g > see[qt]) s[qt][t][i] = -INFINITY;
+            if (16 * t + 4 * i > up_to) s[qt][t][i] = -INFINITY;
       }
-      for (int x = 32; x > 0; x >>= 1) last = max(last, __shfl_xor(last, x));
       // what no query sees may hold anything: nothing of it may reach the sums (0 times what is not finite).  Values that are not
       // numbers and that some see are left out of the product and put where they belong below.
       bool bad = false;
+      const int up_to = last_token - token0 - g;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const unsigned byte = 0xffu << (8 * t);
-          const bool nobody = base + 16 * t + 4 * i + g > last;
-          if (!nobody && (vs[i] & byte) == byte) bad = true;
-          if (nobody || (vs[i] & byte) == byte) vs[i] &= ~byte;
+          const bool nobody = 16 * t + 4 * i > up_to;
+          if (!nobody && (r.vs[i] & byte) == byte) bad = true;
+          if (nobody || (r.vs[i] & byte) == byte) r.vs[i] &= ~byte;
         }
       odd = __ballot(bad) != 0;
     }
@@ -364,15 +430,15 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) voi
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][t][i], prm.scale, -ref));
-          if (part && base + 16 * t + 4 * i + g > see[qt]) e[i] = 0.f;
           l[qt] += e[i];
         }
         // P is rounded to the operands' type: half a step each, without a bias, against sums of the numerators as they are
         p[qt][t >> 1][2 * (t & 1)] = pack2<BF16>(e[0], e[1]);
         p[qt][t >> 1][2 * (t & 1) + 1] = pack2<BF16>(e[2], e[3]);
       }
-      seen[qt] |= !part || see[qt] >= base;
+      if (!part || see[qt] >= token0) marks |= 0x10000u << qt;
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -380,8 +446,7 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) voi
         unsigned x[8][4];                     // of 8 tokens, 4 pairs of columns (2 at D = 64)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = 2 * half + (j >> 2), i = j & 3;
-          const float sc = scale_of(vs[i], t);
+          const float sc = scale_of(r.vs[j & 3], 2 * half + (j >> 2));
           x[j][0] = convert2<BF16, 0>(r.v[8 * half + j][w], sc);
           x[j][1] = convert2<BF16, 1>(r.v[8 * half + j][w], sc);
           if constexpr (D > 64) {
@@ -391,55 +456,42 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) voi
         }
 #pragma unroll
         for (int e = 0; e < (D == 64 ? 2 : 4); ++e) {
-          uintx4 lo, hi;
+          uintx4 low, high;
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            lo[y] = __builtin_amdgcn_perm(x[2 * y + 1][e], x[2 * y][e], 0x05040100u);
-            hi[y] = __builtin_amdgcn_perm(x[2 * y + 1][e], x[2 * y][e], 0x07060302u);
+            low[y] = __builtin_amdgcn_perm(x[2 * y + 1][e], x[2 * y][e], 0x05040100u);
+            high[y] = __builtin_amdgcn_perm(x[2 * y + 1][e], x[2 * y][e], 0x07060302u);
           }
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            o[qt][8 * w + 2 * e] = mfma16<BF16>(lo, p[qt][half], o[qt][8 * w + 2 * e]);
-            o[qt][8 * w + 2 * e + 1] = mfma16<BF16>(hi, p[qt][half], o[qt][8 * w + 2 * e + 1]);
+            o[qt][8 * w + 2 * e] = mfma16<BF16>(low, p[qt][half], o[qt][8 * w + 2 * e]);
+            o[qt][8 * w + 2 * e + 1] = mfma16<BF16>(high, p[qt][half], o[qt][8 * w + 2 * e + 1]);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (odd) {
       // rare: values that are not numbers reach the queries that see their token, all others stay clear of them
-      const uint8_t* bytes = c.v_scales + page_of_head(c, page, h) * page_scales(D);
+      const uint8_t* bytes = c.v_scales + page_of_head(c, this_page, h) * page_scales(D);
       for (int t = 0; t < PAGE; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (bytes[((4 * g + i) * DT / 32) * PAGE + scale_at(t)] != NOT_FINITE) continue;
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
-            if (base + t <= see[qt])
-#pragma unroll
-              for (int x = 0; x < DT; ++x) o[qt][x][i] = __builtin_nanf("");
+            if (token0 + t <= see[qt]) marks |= 1u << (4 * qt + i);
         }
     }
-  };
-
-  {
-    PageRegs<D> now, ahead;
-    int page = 0, index = 0, page1 = 0, index1 = 0;
-    bool more = next(page, index);
-    if (more) load(now, page, index);
-    while (more) {
-      more = next(page1, index1);
-      if (more) load(ahead, page1, index1);
-      take(now, page, index);
-      now = ahead;
-      page = page1; index = index1;
-    }
+    if (!more) break;
+    load_values<D>(r, c, page_of_head(c, page, h), n, g);
   }
 
   // ---- the wavefronts meet ----
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     l[qt] = quad_sum(l[qt]);
-    m[qt] = m[qt] == -INFINITY ? (seen[qt] ? NO_MASS : -INFINITY) : m[qt] * prm.scale - HEADROOM<BF16>;
+    m[qt] = m[qt] == -INFINITY ? ((marks >> (16 + qt) & 1) != 0 ? NO_MASS : -INFINITY) : m[qt] * prm.scale - HEADROOM<BF16>;
     if (g == 0) {
       lds_ml[(wave * ROWS + 16 * qt + n) * 2] = m[qt];
       lds_ml[(wave * ROWS + 16 * qt + n) * 2 + 1] = l[qt];
@@ -460,100 +512,134 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : 2) voi
     const float f = m[qt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[qt] - top);
     float* out = lds + (wave * ROWS + 16 * qt + n) * PITCH;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const float fi = (marks >> (4 * qt + i) & 1) != 0 ? __builtin_nanf("") : f;
 #pragma unroll
       for (int x = 0; x < DT; x += 4)
-        *reinterpret_cast<floatx4*>(out + (4 * g + i) * DT + x) = floatx4{o[qt][x][i] * f, o[qt][x + 1][i] * f, o[qt][x + 2][i] * f, o[qt][x + 3][i] * f};
-  }
-  __syncthreads();
-
-  // result row r of the tile, columns d .. d + 3, not yet divided by the sum
-  const int real_rows = min(ROWS, prm.rows - tile * ROWS);
-  auto put = [&](int r, int d, floatx4 x, float top, float sum) {
-    const int row = tile * ROWS + r, token = row / prm.group, head = h * prm.group + (row - token * prm.group);
-    const bool none = token >= un.count || top == -INFINITY;
-    const float f = none ? 0.f : 1.0f / sum;            // (a row that has seen tokens and has no mass: 0 times infinity, not a number)
-    const int64_t at = b * prm.a.os[0] + head * prm.a.os[1] + token * prm.a.os[2] + d;
-    store_out4<BF16>(prm.a.o, at, prm.a.out_f32 != 0, none ? 0.f : x[0] * f, none ? 0.f : x[1] * f, none ? 0.f : x[2] * f, none ? 0.f : x[3] * f);
-    if (prm.a.lse != nullptr && d == 0)
-      prm.a.lse[((int64_t)b * prm.a.H + head) * prm.a.N + token] = none || sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
-  };
-  constexpr int QUADS = D / 4;
-  float* slot_o = nullptr;
-  if (splits > 1) slot_o = prm.part_o + ((int64_t)(first_wg + split) * c.heads + h) * (ROWS * D);
-  for (int e = threadIdx.x; e < real_rows * QUADS; e += 64 * WAVES) {
-    const int r = e / QUADS, d = 4 * (e % QUADS);
-    floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) x += *reinterpret_cast<const floatx4*>(lds + (w * ROWS + r) * PITCH + d);
-    if (splits == 1) put(r, d, x, lds_row[2 * r], lds_row[2 * r + 1]);
-    else coherent_store4(slot_o + r * D + d, x[0], x[1], x[2], x[3]);
-  }
-  if (splits == 1) return;
-
-  // ---- the workgroups meet ----
-  if (threadIdx.x < 2 * real_rows)
-    coherent_store(prm.part_ml + ((int64_t)(first_wg + split) * c.heads + h) * (ROWS * 2) + threadIdx.x, lds_row[threadIdx.x]);
-  wait_vm<0>();
-  __syncthreads();
-  unsigned long long* arrivals = prm.arrivals + (int64_t)unit * c.heads + h;
-  int* const count = reinterpret_cast<int*>(lds_ml);
-  if (threadIdx.x == 0) *count = count_part(arrivals, prm.epoch);
-  __syncthreads();
-  if (*(volatile int*)count != splits) return;
-  // weights of the parts: [split][row] in the room of the parts of O, found by 256 / ROWS threads a row
-  {
-    constexpr int PER = 64 * WAVES / ROWS;
-    const int r = threadIdx.x / PER, x = threadIdx.x % PER;
-    float top = -INFINITY, sum = 0.f;
-    const float* ml = prm.part_ml + ((int64_t)first_wg * c.heads + h) * (ROWS * 2) + 2 * r;
-    const int64_t step = (int64_t)c.heads * (ROWS * 2);
-    if (r < real_rows) for (int s = x; s < splits; s += PER) top = fmaxf(top, coherent_load(ml + s * step));
-#pragma unroll
-    for (int y = PER / 2; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor(top, y));
-    if (r < real_rows) for (int s = x; s < splits; s += PER) {
-      const float ms = coherent_load(ml + s * step), f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - top);
-      lds[s * ROWS + r] = f;
-      sum += f == 0.f ? 0.f : f * coherent_load(ml + s * step + 1);
+        *reinterpret_cast<floatx4*>(out + (4 * g + i) * DT + x) = floatx4{o[qt][x][i] * fi, o[qt][x + 1][i] * fi, o[qt][x + 2][i] * fi, o[qt][x + 3][i] * fi};
     }
-#pragma unroll
-    for (int y = PER / 2; y > 0; y >>= 1) sum += __shfl_xor(sum, y);
-    if (x == 0) { lds_row[2 * r] = top; lds_row[2 * r + 1] = sum; }
   }
   __syncthreads();
-  {
-    const float* part = prm.part_o + ((int64_t)first_wg * c.heads + h) * (ROWS * D);
-    const int64_t step = (int64_t)c.heads * (ROWS * D);
-    for (int e = threadIdx.x; e < real_rows * QUADS; e += 64 * WAVES) {
+
+  // (from here on the arguments are read again: kept over the pages they would crowd the scalar registers)
+  const ParamsAgain late = params_again();
+  constexpr int QUADS = D / 4;
+  const int real_rows = min(ROWS, late->rows - tile * ROWS);
+  const int cells = real_rows * QUADS;        // a cell: 4 columns of a row
+  // what is added up for the result: parts `parts` x `part_step` floats apart, rows `pitch` apart
+  const float* parts = lds;
+  int parts_n = WAVES, part_step = ROWS * PITCH, pitch = PITCH;
+  bool last_in = true;
+  if (splits > 1) {
+    // ---- the workgroups meet ----
+    // a workgroup has two parts at most: of the unit that goes on from the range in front of it, and of the one that goes on behind it
+    auto slot_of = [&](int x) { return ((int64_t)(first_wg + x) * 2 + (x == 0)) * late->c.heads + h; };
+    float* slot_o = late->part_o + slot_of(split) * (ROWS * D);
+    for (int e = threadIdx.x; e < cells; e += 64 * WAVES) {
       const int r = e / QUADS, d = 4 * (e % QUADS);
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int s = 0; s < splits; ++s) {
-        const float f = lds[s * ROWS + r];
-        const float* from = part + s * step + r * D + d;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += f * coherent_load(from + i);
+      for (int y = 0; y < WAVES; ++y) x += *reinterpret_cast<const floatx4*>(lds + (y * ROWS + r) * PITCH + d);
+      coherent_store4(slot_o + 4 * e, x[0], x[1], x[2], x[3]);
+    }
+    if (threadIdx.x < 2 * real_rows) coherent_store(late->part_ml + slot_of(split) * (ROWS * 2) + threadIdx.x, lds_row[threadIdx.x]);
+    wait_vm<0>();
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      if (threadIdx.x == 0) __hip_atomic_store(late->flags + slot_of(split), late->mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      wait_vm<0>();
+      bool all = true;
+#pragma unroll 4
+      for (int y = lane; y < splits; y += 64) all &= __hip_atomic_load(late->flags + slot_of(y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == late->mark;
+      all = __ballot(!all) == 0;
+      if (threadIdx.x == 0) *reinterpret_cast<int*>(lds_ml) = all;
+    }
+    __syncthreads();
+    last_in = *reinterpret_cast<volatile int*>(lds_ml) != 0;
+    if (last_in) {
+      // 256 / ROWS threads a row find its maximum and its sum ...
+      const int64_t step = 2 * (int64_t)late->c.heads;                           // slots from part to part, but for the first
+      const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2);
+      const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2);
+      {
+        constexpr int PER = 64 * WAVES / ROWS;
+        const int r = threadIdx.x / PER, x = threadIdx.x % PER;
+        float top = -INFINITY, sum = 0.f;
+        if (r < real_rows)
+#pragma unroll 4
+          for (int y = x; y < splits; y += PER) {
+            const floatx2 ml = coherent_load2((y == 0 ? ml0 : ml1 + y * step * (ROWS * 2)) + 2 * r);
+            const float next_top = fmaxf(top, ml[0]);
+            if (ml[0] != -INFINITY) sum = (top == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next_top)) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - next_top);
+            top = next_top;
+          }
+#pragma unroll
+        for (int y = PER / 2; y > 0; y >>= 1) {
+          const float other = __shfl_xor(top, y), more_sum = __shfl_xor(sum, y), next_top = fmaxf(top, other);
+          sum = (top == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next_top)) + (other == -INFINITY ? 0.f : more_sum * __builtin_amdgcn_exp2f(other - next_top));
+          top = next_top;
+        }
+        if (x == 0) { lds_row[2 * r] = top; lds_row[2 * r + 1] = sum; }
       }
-      put(r, d, x, lds_row[2 * r], lds_row[2 * r + 1]);
+      __syncthreads();
+      // ... and the parts of O go to `teams` groups of threads, where there are few rows, which meet in LDS
+      const int teams = max(1, 64 * WAVES / cells);
+      const float* const o0 = late->part_o + slot_of(0) * (ROWS * D);
+      const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D);
+      for (int e0 = threadIdx.x; e0 < cells * teams; e0 += 64 * WAVES) {
+        const int team = e0 / cells, e = e0 - team * cells, r = e / QUADS;
+        const float top = lds_row[2 * r];
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int y = team; y < splits; y += teams) {
+          const float* at_part = (y == 0 ? o0 : o1 + y * step * (ROWS * D)) + 4 * e;
+          const float my = coherent_load((y == 0 ? ml0 : ml1 + y * step * (ROWS * 2)) + 2 * r);
+          const floatx2 x0 = coherent_load2(at_part), x1 = coherent_load2(at_part + 2);
+          const float f = my == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(my - top);
+          x += f * floatx4{x0[0], x0[1], x1[0], x1[1]};
+        }
+        *reinterpret_cast<floatx4*>(lds + 4 * e0) = x;
+      }
+      __syncthreads();
+      parts = lds; parts_n = teams; part_step = 4 * cells; pitch = D;
+      for (int y = threadIdx.x; y < splits; y += 64 * WAVES) __hip_atomic_store(late->flags + slot_of(y), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  // back to zero, so that a replay of this launch (same mark) starts from a clean counter
-  if (threadIdx.x == 0) __hip_atomic_store(arrivals, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (last_in)
+    for (int e = threadIdx.x; e < cells; e += 64 * WAVES) {
+      const int r = e / QUADS, d = 4 * (e % QUADS);
+      const int row = tile * ROWS + r, token = by_group(row, late->group, late->per_group), head = h * late->group + (row - token * late->group);
+      const float top = lds_row[2 * r], sum = lds_row[2 * r + 1];
+      floatx4 x = {0.f, 0.f, 0.f, 0.f};
+      for (int y = 0; y < parts_n; ++y) x += *reinterpret_cast<const floatx4*>(parts + y * part_step + r * pitch + d);
+      const bool none = token >= un.count || top == -INFINITY;
+      const float f = 1.0f / sum;             // (a row that has seen tokens and has no mass: 0 times infinity, not a number)
+      store_out4<BF16>(late->a.o, b * late->a.os[0] + head * late->a.os[1] + token * late->a.os[2] + d, late->a.out_f32 != 0, none ? 0.f : x[0] * f,
+                       none ? 0.f : x[1] * f, none ? 0.f : x[2] * f, none ? 0.f : x[3] * f);
+      if (late->a.lse != nullptr && d == 0)
+        late->a.lse[((int64_t)b * late->a.H + head) * late->a.N + token] = none || sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+    }
+  __syncthreads();                            // (the next unit's parts go where these are)
+  }
+  if (behind >= hi) break;
+  base += 64;
+  }
 }
 
 // ---- host ----
-struct CachePlan { int qt, tiles, W, max_splits; int64_t units; };      // W = 0: a workgroup per (unit, head)
+// W = 0: a workgroup per (unit, head)
+struct CachePlan { int qt, tiles, W; int64_t units; };
 static CachePlan cache_plan(const bsattn_cache& c, int B, int H, int N) {
   CachePlan p;
   const int64_t rows = (int64_t)N * (H / c.heads);
   p.qt = rows <= 16 ? 1 : (rows <= 32 || c.head_dim == 256 ? 2 : 4);
   p.tiles = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
   p.units = (int64_t)B * p.tiles;
-  const int per_cu = p.qt == 1 && c.head_dim < 256 ? 2 : 1;
+  const int per_cu = p.qt == 1 ? (c.head_dim < 256 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
   const int64_t fill = (int64_t)compute_units() * per_cu;
-  p.max_splits = 256 / p.qt;
-  // shared where a workgroup a unit would leave compute units idle or wait for the longest sequence
-  p.W = p.units * c.heads < 4 * fill && p.units <= 1024 ? (int)std::max<int64_t>(1, fill / c.heads) : 0;
+  // ranges where a workgroup a unit would leave compute units idle or wait for the longest sequence (the axis is counted in 32 bits)
+  const bool ranges = p.units * c.heads < 4 * fill && p.units <= 1024 && p.units * ((int64_t)c.max_pages + STEP + GAP<1>) < 0x7fffffffLL;
+  p.W = ranges ? (int)std::max<int64_t>(1, fill / c.heads) : 0;
   return p;
 }
 
@@ -561,22 +647,27 @@ static size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 size_t cache_attn_workspace_bytes(const bsattn_cache& c, int B, int H, int N) {
   const CachePlan p = cache_plan(c, B, H, N);
   if (p.W == 0) return 256;
-  const size_t slots = ((size_t)p.W + p.units) * c.heads, rows = 16 * (size_t)p.qt;
-  return rounded(slots * rows * c.head_dim * 4) + rounded(slots * rows * 8) + rounded((size_t)p.units * c.heads * 8);
+  const size_t slots = 2 * (size_t)p.W * c.heads, rows = 16 * (size_t)p.qt;
+  return rounded(slots * rows * c.head_dim * 4) + rounded(slots * rows * 8) + rounded(slots * 8);
 }
 
-template <int D, bool BF16, int QT>
+template <int D, bool BF16, int QT, bool MASK>
 static void launch_one(const CacheAttnParams& prm, unsigned blocks, hipStream_t st) {
   constexpr int LDS = (WAVES * 16 * QT * (D + 4) + WAVES * 16 * QT * 2 + 16 * QT * 2) * 4;
   static std::atomic<unsigned long long> configured{0};     // raising the dynamic LDS limit is idempotent
-  once_per_device(configured, [] { (void)hipFuncSetAttribute((const void*)cache_attn_kernel<D, BF16, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
-  hipLaunchKernelGGL((cache_attn_kernel<D, BF16, QT>), dim3(blocks), dim3(64 * WAVES), LDS, st, prm);
+  once_per_device(configured, [] { (void)hipFuncSetAttribute((const void*)cache_attn_kernel<D, BF16, QT, MASK>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
+  hipLaunchKernelGGL((cache_attn_kernel<D, BF16, QT, MASK>), dim3(blocks), dim3(64 * WAVES), LDS, st, prm);
+}
+template <int D, bool BF16, int QT>
+static void launch_rows(const CacheAttnParams& prm, unsigned blocks, hipStream_t st) {
+  if (prm.a.mask != nullptr) launch_one<D, BF16, QT, true>(prm, blocks, st);
+  else launch_one<D, BF16, QT, false>(prm, blocks, st);
 }
 template <int D, bool BF16>
-static void launch_rows(const CacheAttnParams& prm, int qt, unsigned blocks, hipStream_t st) {
-  if (qt == 1) launch_one<D, BF16, 1>(prm, blocks, st);
-  else if (D == 256 || qt == 2) launch_one<D, BF16, 2>(prm, blocks, st);
-  else if constexpr (D != 256) launch_one<D, BF16, 4>(prm, blocks, st);
+static void launch_tiles(const CacheAttnParams& prm, int qt, unsigned blocks, hipStream_t st) {
+  if (qt == 1) launch_rows<D, BF16, 1>(prm, blocks, st);
+  else if (D == 256 || qt == 2) launch_rows<D, BF16, 2>(prm, blocks, st);
+  else if constexpr (D != 256) launch_rows<D, BF16, 4>(prm, blocks, st);
 }
 
 int launch_cache_attn(const bsattn_cache& c, const CacheAttn& a, void* ws, hipStream_t st) {
@@ -585,25 +676,26 @@ int launch_cache_attn(const bsattn_cache& c, const CacheAttn& a, void* ws, hipSt
   prm.c = c; prm.a = a;
   prm.group = a.H / c.heads;
   prm.rows = a.N * prm.group;
+  prm.per_group = prm.group > 1 ? 0xffffffffu / prm.group + 1u : 0u;
   prm.tiles = p.tiles;
-  prm.W = p.W; prm.max_splits = p.max_splits;
-  prm.min_pages = WAVES;
-  prm.scale = fabsf(a.sm_scale) * LOG2E;
+  prm.W = p.W;
+  // (not 0: a score of -inf, which stands for a token that is not seen, stays one)
+  prm.scale = std::max(fabsf(a.sm_scale) * LOG2E, FLT_MIN);
   prm.flip = a.sm_scale < 0.f ? 0x80008000u : 0u;
   if (p.W > 0) {
-    const size_t slots = ((size_t)p.W + p.units) * c.heads, rows = 16 * (size_t)p.qt;
+    const size_t slots = 2 * (size_t)p.W * c.heads, rows = 16 * (size_t)p.qt;
     char* at = (char*)ws;
     prm.part_o = (float*)at; at += rounded(slots * rows * c.head_dim * 4);
     prm.part_ml = (float*)at; at += rounded(slots * rows * 8);
-    prm.arrivals = (unsigned long long*)at;
-    prm.epoch = next_epoch();
+    prm.flags = (unsigned long long*)at;
+    prm.mark = next_epoch();
   }
-  const int64_t blocks = (p.W + p.units) * c.heads;
+  const int64_t blocks = (p.W > 0 ? p.W : p.units) * c.heads;
   if (blocks > 0x7fffffffLL) return BSATTN_ERR_RANGE;
   const bool bf16 = c.dtype == BSATTN_BF16;
-  if (c.head_dim == 64) bf16 ? launch_rows<64, true>(prm, p.qt, (unsigned)blocks, st) : launch_rows<64, false>(prm, p.qt, (unsigned)blocks, st);
-  else if (c.head_dim == 128) bf16 ? launch_rows<128, true>(prm, p.qt, (unsigned)blocks, st) : launch_rows<128, false>(prm, p.qt, (unsigned)blocks, st);
-  else bf16 ? launch_rows<256, true>(prm, p.qt, (unsigned)blocks, st) : launch_rows<256, false>(prm, p.qt, (unsigned)blocks, st);
+  if (c.head_dim == 64) bf16 ? launch_tiles<64, true>(prm, p.qt, (unsigned)blocks, st) : launch_tiles<64, false>(prm, p.qt, (unsigned)blocks, st);
+  else if (c.head_dim == 128) bf16 ? launch_tiles<128, true>(prm, p.qt, (unsigned)blocks, st) : launch_tiles<128, false>(prm, p.qt, (unsigned)blocks, st);
+  else bf16 ? launch_tiles<256, true>(prm, p.qt, (unsigned)blocks, st) : launch_tiles<256, false>(prm, p.qt, (unsigned)blocks, st);
   return launch_status();
 }
 
