@@ -36,6 +36,7 @@
 namespace bsattn {
 
 constexpr int WAVES = 4;
+constexpr int MERGE = 16;                     // parts that a thread asks for at a time
 constexpr int STEP = 16;                      // (see above)
 // Pages of the shortest range, and how near to a unit's end a cut goes there; a tile of more rows takes as much longer for a page.
 // (Fewer than GAP positions are never between two cuts, so that one cut at most is near an end.)
@@ -73,6 +74,11 @@ __device__ __forceinline__ ParamsAgain params_again() {
   ParamsAgain p = (ParamsAgain)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return p;
+}
+
+__device__ __forceinline__ void coherent_store2(float* p, float a, float b) {
+  const floatx2 x = {a, b};
+  __hip_atomic_store((unsigned long long*)p, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Sum over the lanes up to this one
@@ -191,15 +197,33 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& prm, int b, int t
   return u;
 }
 
+// Floats of LDS for the (m, l) of parts that meet there: four wavefronts' for each row, or those of a thread each 4 columns
+template <int D, int QT> constexpr int ML_FLOATS = WAVES * 16 * QT * 2 > 2 * (64 * WAVES / (D / 4)) ? WAVES * 16 * QT * 2 : 2 * (64 * WAVES / (D / 4));
+
+// Adds a part of a row (its reference exponent m, its sum l, 4 columns y) to what (top, sum, x) have of it
+__device__ __forceinline__ void merge(float& top, float& sum, floatx4& x, float m, float l, floatx4 y) {
+  const float high = fmaxf(top, m);
+  const float a = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - high), b = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - high);
+  sum = sum * a + l * b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = x[i] * a + y[i] * b;
+  top = high;
+}
+
+// Workgroups of a compute unit (and wavefronts of a SIMD): what the registers leave room for
+template <int D, int QT> constexpr int PER_CU = D * QT >= 512 || QT == 4 ? 1 : (QT == 1 && D <= 128 ? 3 : 2);
+
 template <int D, bool BF16, int QT, bool MASK>
-__global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT == 1 && D <= 128 ? 3 : 2)) void cache_attn_kernel(const CacheAttnParams prm) {
+__global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel(const CacheAttnParams prm) {
   constexpr int ROWS = 16 * QT, PITCH = D + 4, KSTEPS = D / 32, DT = D / 16;
-  extern __shared__ __align__(16) float lds[];           // [WAVES][ROWS][PITCH] parts of O | [WAVES][ROWS][2] (m, l) | [ROWS][2]
+  extern __shared__ __align__(16) float lds[];           // [WAVES][ROWS][PITCH] parts of O | their (m, l) | 1 word
   float* const lds_ml = lds + WAVES * ROWS * PITCH;
-  float* const lds_row = lds_ml + WAVES * ROWS * 2;
+  volatile int* const lds_last = reinterpret_cast<int*>(lds_ml + ML_FLOATS<D, QT>);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const bsattn_cache& c = prm.c;
-  const int h = blockIdx.x % (unsigned)c.heads, w = blockIdx.x / (unsigned)c.heads;
+  const int w = blockIdx.x / (unsigned)c.heads;
+  // (the ranges of a head go to all XCDs, which are not equally near to all memory; tiles of one sequence share an L2's copy of its pages)
+  const int h = prm.W > 0 && prm.tiles == 1 ? (blockIdx.x + w) % (unsigned)c.heads : blockIdx.x - w * c.heads;
   const int units = prm.a.B * prm.tiles;
   // positions of a unit's pages on the axis
   auto positions = [&](int pages) { return MASK ? (pages + STEP - 1) / STEP * STEP : pages; };
@@ -351,7 +375,15 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
     load_values<D>(r, c, page_of_head(c, page, h), n, g);
     load_kept();
   }
+  int turn = 4 * __builtin_amdgcn_s_getreg(4 | 3 << 11);       // the wavefront's place on its SIMD (HW_ID, bits 0 .. 3)
   while (more) {
+    // Of the wavefronts of a SIMD the one that came first would be served first, and end up to a fifth earlier: they take turns
+    if constexpr (PER_CU<D, QT> > 1) {
+      const int now = (++turn >> 2) % PER_CU<D, QT>;
+      if (now == 0) __builtin_amdgcn_s_setprio(0);
+      else if (now == 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(2);
+    }
     const int token0 = index * PAGE, this_page = page;
     floatx4 s[QT][4];
 #pragma unroll
@@ -488,35 +520,28 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
   }
 
   // ---- the wavefronts meet ----
+  const int tile_rows = min(ROWS, prm.rows - tile * ROWS);
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     l[qt] = quad_sum(l[qt]);
     m[qt] = m[qt] == -INFINITY ? ((marks >> (16 + qt) & 1) != 0 ? NO_MASS : -INFINITY) : m[qt] * prm.scale - HEADROOM<BF16>;
     if (g == 0) {
-      lds_ml[(wave * ROWS + 16 * qt + n) * 2] = m[qt];
-      lds_ml[(wave * ROWS + 16 * qt + n) * 2 + 1] = l[qt];
+      if (16 * qt + n < tile_rows) {
+        lds_ml[2 * (wave * tile_rows + 16 * qt + n)] = m[qt];
+        lds_ml[2 * (wave * tile_rows + 16 * qt + n) + 1] = l[qt];
+      }
     }
   }
-  __syncthreads();
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[(w * ROWS + 16 * qt + n) * 2]);
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float mw = lds_ml[(w * ROWS + 16 * qt + n) * 2];
-      if (mw != -INFINITY) sum += lds_ml[(w * ROWS + 16 * qt + n) * 2 + 1] * __builtin_amdgcn_exp2f(mw - top);
-    }
-    if (wave == 0 && g == 0) { lds_row[(16 * qt + n) * 2] = top; lds_row[(16 * qt + n) * 2 + 1] = sum; }
-    const float f = m[qt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[qt] - top);
     float* out = lds + (wave * ROWS + 16 * qt + n) * PITCH;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float fi = (marks >> (4 * qt + i) & 1) != 0 ? __builtin_nanf("") : f;
+      const bool odd = (marks >> (4 * qt + i) & 1) != 0;
 #pragma unroll
       for (int x = 0; x < DT; x += 4)
-        *reinterpret_cast<floatx4*>(out + (4 * g + i) * DT + x) = floatx4{o[qt][x][i] * fi, o[qt][x + 1][i] * fi, o[qt][x + 2][i] * fi, o[qt][x + 3][i] * fi};
+        *reinterpret_cast<floatx4*>(out + (4 * g + i) * DT + x) =
+            odd ? floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")} : floatx4{o[qt][x][i], o[qt][x + 1][i], o[qt][x + 2][i], o[qt][x + 3][i]};
     }
   }
   __syncthreads();
@@ -526,8 +551,7 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
   constexpr int QUADS = D / 4;
   const int real_rows = min(ROWS, late->rows - tile * ROWS);
   const int cells = real_rows * QUADS;        // a cell: 4 columns of a row
-  // what is added up for the result: parts `parts` x `part_step` floats apart, rows `pitch` apart
-  const float* parts = lds;
+  // what is added up for the result: parts `part_step` floats apart, rows `pitch` apart, their references and sums in lds_ml
   int parts_n = WAVES, part_step = ROWS * PITCH, pitch = PITCH;
   bool last_in = true;
   if (splits > 1) {
@@ -538,11 +562,13 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
     for (int e = threadIdx.x; e < cells; e += 64 * WAVES) {
       const int r = e / QUADS, d = 4 * (e % QUADS);
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int y = 0; y < WAVES; ++y) x += *reinterpret_cast<const floatx4*>(lds + (y * ROWS + r) * PITCH + d);
+      for (int y = 0; y < WAVES; ++y)
+        merge(top, sum, x, lds_ml[2 * (y * real_rows + r)], lds_ml[2 * (y * real_rows + r) + 1], *reinterpret_cast<const floatx4*>(lds + (y * ROWS + r) * PITCH + d));
       coherent_store4(slot_o + 4 * e, x[0], x[1], x[2], x[3]);
+      if (d == 0) coherent_store2(late->part_ml + slot_of(split) * (ROWS * 2) + 2 * r, top, sum);
     }
-    if (threadIdx.x < 2 * real_rows) coherent_store(late->part_ml + slot_of(split) * (ROWS * 2) + threadIdx.x, lds_row[threadIdx.x]);
     wait_vm<0>();
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -552,56 +578,34 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
 #pragma unroll 4
       for (int y = lane; y < splits; y += 64) all &= __hip_atomic_load(late->flags + slot_of(y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == late->mark;
       all = __ballot(!all) == 0;
-      if (threadIdx.x == 0) *reinterpret_cast<int*>(lds_ml) = all;
+      if (threadIdx.x == 0) *lds_last = all;
     }
     __syncthreads();
-    last_in = *reinterpret_cast<volatile int*>(lds_ml) != 0;
+    last_in = *lds_last != 0;
     if (last_in) {
-      // 256 / ROWS threads a row find its maximum and its sum ...
+      // The parts go to `teams` groups of threads, where there are few rows; the groups meet in LDS
       const int64_t step = 2 * (int64_t)late->c.heads;                           // slots from part to part, but for the first
-      const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2);
-      const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2);
-      {
-        constexpr int PER = 64 * WAVES / ROWS;
-        const int r = threadIdx.x / PER, x = threadIdx.x % PER;
-        float top = -INFINITY, sum = 0.f;
-        if (r < real_rows)
-#pragma unroll 4
-          for (int y = x; y < splits; y += PER) {
-            const floatx2 ml = coherent_load2((y == 0 ? ml0 : ml1 + y * step * (ROWS * 2)) + 2 * r);
-            const float next_top = fmaxf(top, ml[0]);
-            if (ml[0] != -INFINITY) sum = (top == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next_top)) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - next_top);
-            top = next_top;
-          }
-#pragma unroll
-        for (int y = PER / 2; y > 0; y >>= 1) {
-          const float other = __shfl_xor(top, y), more_sum = __shfl_xor(sum, y), next_top = fmaxf(top, other);
-          sum = (top == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next_top)) + (other == -INFINITY ? 0.f : more_sum * __builtin_amdgcn_exp2f(other - next_top));
-          top = next_top;
-        }
-        if (x == 0) { lds_row[2 * r] = top; lds_row[2 * r + 1] = sum; }
-      }
-      __syncthreads();
-      // ... and the parts of O go to `teams` groups of threads, where there are few rows, which meet in LDS
       const int teams = max(1, 64 * WAVES / cells);
-      const float* const o0 = late->part_o + slot_of(0) * (ROWS * D);
-      const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D);
       for (int e0 = threadIdx.x; e0 < cells * teams; e0 += 64 * WAVES) {
         const int team = e0 / cells, e = e0 - team * cells, r = e / QUADS;
-        const float top = lds_row[2 * r];
+        const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2) + 2 * r;
+        const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2) + 2 * r;
+        const float* const o0 = late->part_o + slot_of(0) * (ROWS * D) + 4 * e;
+        const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D) + 4 * e;
         floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll MERGE
         for (int y = team; y < splits; y += teams) {
-          const float* at_part = (y == 0 ? o0 : o1 + y * step * (ROWS * D)) + 4 * e;
-          const float my = coherent_load((y == 0 ? ml0 : ml1 + y * step * (ROWS * 2)) + 2 * r);
+          const float* at_part = y == 0 ? o0 : o1 + y * step * (ROWS * D);
+          const floatx2 ml = coherent_load2(y == 0 ? ml0 : ml1 + y * step * (ROWS * 2));
           const floatx2 x0 = coherent_load2(at_part), x1 = coherent_load2(at_part + 2);
-          const float f = my == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(my - top);
-          x += f * floatx4{x0[0], x0[1], x1[0], x1[1]};
+          merge(top, sum, x, ml[0], ml[1], floatx4{x0[0], x0[1], x1[0], x1[1]});
         }
         *reinterpret_cast<floatx4*>(lds + 4 * e0) = x;
+        if (e % QUADS == 0) { lds_ml[2 * (team * real_rows + r)] = top; lds_ml[2 * (team * real_rows + r) + 1] = sum; }
       }
       __syncthreads();
-      parts = lds; parts_n = teams; part_step = 4 * cells; pitch = D;
+      parts_n = teams; part_step = 4 * cells; pitch = D;
       for (int y = threadIdx.x; y < splits; y += 64 * WAVES) __hip_atomic_store(late->flags + slot_of(y), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
@@ -609,9 +613,10 @@ __global__ __launch_bounds__(64 * WAVES, (D * QT >= 512 || QT == 4) ? 1 : (QT ==
     for (int e = threadIdx.x; e < cells; e += 64 * WAVES) {
       const int r = e / QUADS, d = 4 * (e % QUADS);
       const int row = tile * ROWS + r, token = by_group(row, late->group, late->per_group), head = h * late->group + (row - token * late->group);
-      const float top = lds_row[2 * r], sum = lds_row[2 * r + 1];
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
-      for (int y = 0; y < parts_n; ++y) x += *reinterpret_cast<const floatx4*>(parts + y * part_step + r * pitch + d);
+      float top = -INFINITY, sum = 0.f;
+      for (int y = 0; y < parts_n; ++y)
+        merge(top, sum, x, lds_ml[2 * (y * real_rows + r)], lds_ml[2 * (y * real_rows + r) + 1], *reinterpret_cast<const floatx4*>(lds + y * part_step + r * pitch + d));
       const bool none = token >= un.count || top == -INFINITY;
       const float f = 1.0f / sum;             // (a row that has seen tokens and has no mass: 0 times infinity, not a number)
       store_out4<BF16>(late->a.o, b * late->a.os[0] + head * late->a.os[1] + token * late->a.os[2] + d, late->a.out_f32 != 0, none ? 0.f : x[0] * f,
@@ -653,7 +658,7 @@ size_t cache_attn_workspace_bytes(const bsattn_cache& c, int B, int H, int N) {
 
 template <int D, bool BF16, int QT, bool MASK>
 static void launch_one(const CacheAttnParams& prm, unsigned blocks, hipStream_t st) {
-  constexpr int LDS = (WAVES * 16 * QT * (D + 4) + WAVES * 16 * QT * 2 + 16 * QT * 2) * 4;
+  constexpr int LDS = (WAVES * 16 * QT * (D + 4) + ML_FLOATS<D, QT> + 4) * 4;
   static std::atomic<unsigned long long> configured{0};     // raising the dynamic LDS limit is idempotent
   once_per_device(configured, [] { (void)hipFuncSetAttribute((const void*)cache_attn_kernel<D, BF16, QT, MASK>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
   hipLaunchKernelGGL((cache_attn_kernel<D, BF16, QT, MASK>), dim3(blocks), dim3(64 * WAVES), LDS, st, prm);
