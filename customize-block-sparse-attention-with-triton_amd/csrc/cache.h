@@ -41,6 +41,17 @@ __device__ __forceinline__ int length_of(const bsattn_cache& c, int s) {
 // Where a head's page begins, in heads' pages
 __device__ __forceinline__ int64_t page_of_head(const bsattn_cache& c, int page, int h) { return (int64_t)page * c.heads + h; }
 
+// Sum over the lanes up to this one
+__device__ __forceinline__ int wave_upto(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);       // lanes 1, 2, 4, 8 further down in a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);       // a row's last lane to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);       // lane 31 to the upper rows
+  return x;
+}
+
 struct CacheAttn {
   const void* q; void* o; float* lse;
   const uint8_t* mask; int64_t ms[4];                // strides of the mask's batch, heads, blocks of 64 queries, pages (0: one for all)
@@ -59,7 +70,7 @@ struct CacheAppend {
   const int32_t *sequences, *at, *counts;
   int B, N;
 };
-size_t cache_append_workspace_bytes(const bsattn_cache& c, int B, int N);
+size_t cache_append_workspace_bytes(int B, int N);
 int launch_cache_append(const bsattn_cache& c, const CacheAppend& a, void* ws, hipStream_t st);
 int launch_cache_read(const bsattn_cache& c, void* k, void* v, const int64_t* ks, const int64_t* vs, const int32_t* sequences,
                       const int32_t* start, int B, int N, hipStream_t st);

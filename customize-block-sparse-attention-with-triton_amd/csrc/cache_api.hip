@@ -39,8 +39,8 @@ int bsattn_cache_append_workspace(const bsattn_cache* cache, int B, int N, size_
   if (const int rc = check_cache(cache); rc != BSATTN_OK) return rc;
   if (bytes == nullptr) return BSATTN_ERR_NULL;
   if (B <= 0 || N < 0) return BSATTN_ERR_SHAPE;
-  if (B > CACHE_ROWS_MAX || N > cache->max_pages * PAGE || (int64_t)B * cache->max_pages > 0x7fffffffLL) return BSATTN_ERR_RANGE;
-  *bytes = cache_append_workspace_bytes(*cache, B, N);
+  if (B > CACHE_ROWS_MAX || N > cache->max_pages * PAGE || (int64_t)B * (N / PAGE + 2) > 0x7fffffffLL) return BSATTN_ERR_RANGE;
+  *bytes = cache_append_workspace_bytes(B, N);
   return BSATTN_OK;
 }
 
@@ -79,7 +79,7 @@ int bsattn_cache_attn_workspace(const bsattn_cache* cache, int B, int H, int N, 
   if (B <= 0 || H <= 0 || N <= 0 || H % cache->heads != 0) return BSATTN_ERR_SHAPE;
   // rows of a tile are told apart with products of 32 bits
   const int64_t group = H / cache->heads;
-  if (N * group > 0x3fffffffLL || N * group > 0xffffffffLL / group || (int64_t)B * H * N > 0x7fffffffLL) return BSATTN_ERR_RANGE;
+  if (N * group > 0x3fffffffLL || N * group > 0xffffffffLL / group || (int64_t)B * H * N > 0x7fffffffLL || N * group / 16 + 1 > 0xffffffffLL / B / B) return BSATTN_ERR_RANGE;
   *bytes = cache_attn_workspace_bytes(*cache, B, H, N);
   return BSATTN_OK;
 }

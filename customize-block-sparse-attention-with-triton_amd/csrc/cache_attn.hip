@@ -29,6 +29,7 @@
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 #include "common.h"
 #include "kernel_util.h"
 #include "cache.h"
@@ -38,11 +39,10 @@ namespace bsattn {
 constexpr int WAVES = 4;
 constexpr int MERGE = 16;                     // parts that a thread asks for at a time
 constexpr int STEP = 16;                      // (see above)
-// Pages of the shortest range, and how near to a unit's end a cut goes there; a tile of more rows takes as much longer for a page.
-// (Fewer than GAP positions are never between two cuts, so that one cut at most is near an end.)
-template <int QT> constexpr int LEAST = QT == 1 ? 8 : 4;
-template <int QT> constexpr int NEAR = QT == 1 ? 6 : 3;
-template <int QT> constexpr int GAP = NEAR<QT> + 1;
+// Pages of the shortest range (parts cost more to merge than pages to walk), and how near to a unit's end a cut goes there.  (Two cuts
+// are always more than NEAR positions apart: one at most is near an end.)
+template <int D, int QT> constexpr int LEAST = QT == 1 && D < 256 ? 8 : (QT == 1 ? 12 : 8);
+constexpr int NEAR = 6, GAP = NEAR + 1;
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 // Numerators are 2^HEADROOM at most: in fp16, whose steps are equal below 2^-14, small ones keep their digits 15 powers of two further
 // down (without it weights of 2^-16 beside one of 1 were 2^-9 off).
@@ -53,6 +53,7 @@ struct CacheAttnParams {
   bsattn_cache c;
   CacheAttn a;
   int group, rows, tiles, W;      // query heads per head of the cache; N * group; tiles of them; workgroups of a head (0: one a unit)
+  unsigned per_row;               // 2^32 / a.B rounded up (by_group)
   unsigned per_group;             // 2^32 / group rounded up (by_group)
   float scale; unsigned flip;                            // |sm_scale| log2 e; sign bits if sm_scale < 0
   float *part_o, *part_ml;
@@ -79,17 +80,6 @@ __device__ __forceinline__ ParamsAgain params_again() {
 __device__ __forceinline__ void coherent_store2(float* p, float a, float b) {
   const floatx2 x = {a, b};
   __hip_atomic_store((unsigned long long*)p, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// Sum over the lanes up to this one
-__device__ __forceinline__ int wave_upto(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);       // lanes 1, 2, 4, 8 further down in a row of 16
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);       // a row's last lane to the next row
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);       // lane 31 to the upper rows
-  return x;
 }
 
 template <bool BF16>
@@ -191,7 +181,11 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& prm, int b, int t
     return u;
   }
   u.first = length_of(prm.c, u.seq) - u.count;
-  const int t0 = by_group(tile * ROWS, prm.group, prm.per_group), t1 = by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group);
+  int t0 = 0, t1 = prm.a.N - 1;
+  if (prm.tiles > 1) {
+    t0 = by_group(tile * ROWS, prm.group, prm.per_group);
+    t1 = by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group);
+  }
   const int last = u.first + min(u.count - 1, t1);
   u.pages = t0 < u.count && last >= 0 ? last / PAGE + 1 : 0;
   return u;
@@ -211,7 +205,7 @@ __device__ __forceinline__ void merge(float& top, float& sum, floatx4& x, float 
 }
 
 // Workgroups of a compute unit (and wavefronts of a SIMD): what the registers leave room for
-template <int D, int QT> constexpr int PER_CU = D * QT >= 512 || QT == 4 ? 1 : (QT == 1 && D <= 128 ? 3 : 2);
+template <int D, int QT> constexpr int PER_CU = D * QT >= 512 || QT == 4 ? 1 : (QT == 1 && D < 128 ? 3 : 2);
 
 template <int D, bool BF16, int QT, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel(const CacheAttnParams prm) {
@@ -243,8 +237,9 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   length = 0;
   const int lane_unit = base + lane;
   if (prm.W > 0 ? lane_unit < units : lane == 0) {
-    mine = unit_of<ROWS>(prm, lane_unit % prm.a.B, prm.tiles - 1 - lane_unit / prm.a.B);
-    length = positions(mine.pages) + GAP<QT>;
+    const int tile_back = prm.tiles == 1 ? 0 : by_group(lane_unit, prm.a.B, prm.per_row);
+    mine = unit_of<ROWS>(prm, lane_unit - tile_back * prm.a.B, prm.tiles - 1 - tile_back);
+    length = positions(mine.pages) + GAP;
   }
   const int upto = wave_upto(length);
   begin = behind + upto - length;
@@ -254,7 +249,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     total = behind;
     hi = total;
     if (prm.W > 0) {
-      const int ranges = min(prm.W, max(units, total / LEAST<QT>));
+      const int ranges = min(prm.W, max(units, total / (LEAST<D, QT>)));
       if (w >= ranges) return;
       // the first `longer` ranges are one position longer than `each`
       each = (unsigned)total / (unsigned)ranges; longer = total - each * ranges;
@@ -265,7 +260,8 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     if (base > 0 && prm.W > 0) { base = 0; behind = 0; continue; }
   }
   for (unsigned long long mates = __ballot(length > 0 && begin < hi && begin + length > lo); mates != 0; mates &= mates - 1) {
-  const int at = __builtin_ctzll(mates), unit = base + at, b = unit % prm.a.B, tile = prm.tiles - 1 - unit / prm.a.B;
+  const int at = __builtin_ctzll(mates), unit = base + at, unit_back = prm.tiles == 1 ? 0 : by_group(unit, prm.a.B, prm.per_row);
+  const int b = unit - unit_back * prm.a.B, tile = prm.tiles - 1 - unit_back;
   const Unit un = {__builtin_amdgcn_readlane(mine.seq, at), __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.count, at),
                    __builtin_amdgcn_readlane(mine.pages, at)};
   const int unit_begin = __builtin_amdgcn_readlane(begin, at), unit_positions = positions(un.pages);
@@ -273,8 +269,8 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   if (prm.W > 0) {
     first_wg = holder(unit_begin);
     last_wg = unit_positions > 0 ? holder(unit_begin + unit_positions - 1) : first_wg;
-    if (first_wg < last_wg && cut_at(first_wg + 1) - unit_begin <= NEAR<QT>) ++first_wg;
-    if (first_wg < last_wg && unit_begin + unit_positions - cut_at(last_wg) <= NEAR<QT>) --last_wg;
+    if (first_wg < last_wg && cut_at(first_wg + 1) - unit_begin <= NEAR) ++first_wg;
+    if (first_wg < last_wg && unit_begin + unit_positions - cut_at(last_wg) <= NEAR) --last_wg;
     if (w < first_wg || w > last_wg) continue;
   }
   const int splits = last_wg - first_wg + 1, split = w - first_wg;
@@ -586,24 +582,58 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       // The parts go to `teams` groups of threads, where there are few rows; the groups meet in LDS
       const int64_t step = 2 * (int64_t)late->c.heads;                           // slots from part to part, but for the first
       const int teams = max(1, 64 * WAVES / cells);
-      for (int e0 = threadIdx.x; e0 < cells * teams; e0 += 64 * WAVES) {
-        const int team = e0 / cells, e = e0 - team * cells, r = e / QUADS;
-        const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2) + 2 * r;
-        const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2) + 2 * r;
-        const float* const o0 = late->part_o + slot_of(0) * (ROWS * D) + 4 * e;
-        const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D) + 4 * e;
-        floatx4 x = {0.f, 0.f, 0.f, 0.f};
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll MERGE
-        for (int y = team; y < splits; y += teams) {
-          const float* at_part = y == 0 ? o0 : o1 + y * step * (ROWS * D);
-          const floatx2 ml = coherent_load2(y == 0 ? ml0 : ml1 + y * step * (ROWS * 2));
-          const floatx2 x0 = coherent_load2(at_part), x1 = coherent_load2(at_part + 2);
-          merge(top, sum, x, ml[0], ml[1], floatx4{x0[0], x0[1], x1[0], x1[1]});
+      const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2);
+      const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2);
+      const float* const o0 = late->part_o + slot_of(0) * (ROWS * D);
+      const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D);
+      // CELLS cells of a thread at a time, and MERGE / CELLS parts of each
+      auto add_up = [&](auto count) {
+        constexpr int CELLS = decltype(count)::value, PARTS = MERGE / CELLS;
+        for (int e0 = threadIdx.x; e0 < cells * teams; e0 += 64 * WAVES * CELLS) {
+          const int team = e0 / cells;          // (0 where there is more than one cell a thread)
+          int cell[CELLS];
+          floatx4 x[CELLS];
+          float top[CELLS], sum[CELLS];
+#pragma unroll
+          for (int k = 0; k < CELLS; ++k) {
+            cell[k] = min(e0 - team * cells + 64 * WAVES * k, cells - 1);
+            x[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+            top[k] = -INFINITY; sum[k] = 0.f;
+          }
+          for (int y0 = team; y0 < splits; y0 += teams * PARTS) {
+            floatx2 ml[PARTS][CELLS], x0[PARTS][CELLS], x1[PARTS][CELLS];
+#pragma unroll
+            for (int j = 0; j < PARTS; ++j) {
+              const int y = min(y0 + j * teams, splits - 1);
+              const float* at_part = y == 0 ? o0 : o1 + y * step * (ROWS * D);
+              const float* at_ml = y == 0 ? ml0 : ml1 + y * step * (ROWS * 2);
+#pragma unroll
+              for (int k = 0; k < CELLS; ++k) {
+                ml[j][k] = coherent_load2(at_ml + 2 * (cell[k] / QUADS));
+                x0[j][k] = coherent_load2(at_part + 4 * cell[k]);
+                x1[j][k] = coherent_load2(at_part + 4 * cell[k] + 2);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < PARTS; ++j)
+              if (y0 + j * teams < splits)
+#pragma unroll
+                for (int k = 0; k < CELLS; ++k)
+                  merge(top[k], sum[k], x[k], ml[j][k][0], ml[j][k][1], floatx4{x0[j][k][0], x0[j][k][1], x1[j][k][0], x1[j][k][1]});
+          }
+#pragma unroll
+          for (int k = 0; k < CELLS; ++k) {
+            if (e0 + 64 * WAVES * k >= cells * teams) break;
+            *reinterpret_cast<floatx4*>(lds + 4 * (e0 + 64 * WAVES * k)) = x[k];
+            if (cell[k] % QUADS == 0) {
+              lds_ml[2 * (team * real_rows + cell[k] / QUADS)] = top[k];
+              lds_ml[2 * (team * real_rows + cell[k] / QUADS) + 1] = sum[k];
+            }
+          }
         }
-        *reinterpret_cast<floatx4*>(lds + 4 * e0) = x;
-        if (e % QUADS == 0) { lds_ml[2 * (team * real_rows + r)] = top; lds_ml[2 * (team * real_rows + r) + 1] = sum; }
-      }
+      };
+      if (cells <= 64 * WAVES) add_up(std::integral_constant<int, 1>{});
+      else add_up(std::integral_constant<int, 4>{});
       __syncthreads();
       parts_n = teams; part_step = 4 * cells; pitch = D;
       for (int y = threadIdx.x; y < splits; y += 64 * WAVES) __hip_atomic_store(late->flags + slot_of(y), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -640,10 +670,10 @@ static CachePlan cache_plan(const bsattn_cache& c, int B, int H, int N) {
   p.qt = rows <= 16 ? 1 : (rows <= 32 || c.head_dim == 256 ? 2 : 4);
   p.tiles = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
   p.units = (int64_t)B * p.tiles;
-  const int per_cu = p.qt == 1 ? (c.head_dim < 256 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
+  const int per_cu = p.qt == 1 ? (c.head_dim < 128 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
   const int64_t fill = (int64_t)compute_units() * per_cu;
   // ranges where a workgroup a unit would leave compute units idle or wait for the longest sequence (the axis is counted in 32 bits)
-  const bool ranges = p.units * c.heads < 4 * fill && p.units <= 1024 && p.units * ((int64_t)c.max_pages + STEP + GAP<1>) < 0x7fffffffLL;
+  const bool ranges = p.units * c.heads < 4 * fill && p.units <= 1024 && p.units * ((int64_t)c.max_pages + STEP + GAP) < 0x7fffffffLL;
   p.W = ranges ? (int)std::max<int64_t>(1, fill / c.heads) : 0;
   return p;
 }
@@ -681,6 +711,7 @@ int launch_cache_attn(const bsattn_cache& c, const CacheAttn& a, void* ws, hipSt
   prm.c = c; prm.a = a;
   prm.group = a.H / c.heads;
   prm.rows = a.N * prm.group;
+  prm.per_row = a.B > 1 ? 0xffffffffu / a.B + 1u : 0u;
   prm.per_group = prm.group > 1 ? 0xffffffffu / prm.group + 1u : 0u;
   prm.tiles = p.tiles;
   prm.W = p.W;

@@ -5,22 +5,22 @@
 // launch over the whole GPU.  No result depends on the pace of anything: the counters are sums, and what free pages there are is read
 // from the numbers of holders, not from a list.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include "common.h"
 #include "kernel_util.h"
 #include "cache.h"
 
 namespace bsattn {
 
-constexpr int PLAN = 1024;            // threads of a workgroup that decides
+constexpr int PLAN = 1024;            // threads of a workgroup that decides, at most
 
-// Exclusive sum over the workgroup's PLAN threads; total: of all.  scratch: 17 words of LDS.
+// Exclusive sum over the workgroup's T threads; total: of all.  scratch: T / 64 words of LDS.
+template <int T>
 __device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int upto = x;
-#pragma unroll
-  for (int y = 1; y < 64; y <<= 1) {
-    const int z = __shfl_up(upto, y);
-    if (lane >= y) upto += z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, upto = wave_upto(x);
+  if constexpr (T == 64) {
+    total = __builtin_amdgcn_readlane(upto, 63);
+    return upto - x;
   }
   __syncthreads();                    // (the scratch of the scan before has been read)
   if (lane == 63) scratch[wave] = upto;
@@ -28,7 +28,7 @@ __device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < PLAN / 64; ++w) {
+  for (int w = 0; w < T / 64; ++w) {
     const int z = scratch[w];
     before += w < wave ? z : 0;
     total += z;
@@ -36,16 +36,28 @@ __device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
   return before + upto - x;
 }
 
+// An entry of the page table gives its page up
+__device__ __forceinline__ void give_up(const bsattn_cache& c, int32_t* entry) {
+  const int page = *entry;
+  *entry = -1;
+  if (page < 0 || page >= c.pages) report(c.status, STATUS_PAGE);
+  else if (atomicSub(&c.refs[page], 1) == 1) atomicMin(c.free_from, page);
+}
+
 // ---- append ----
 struct AppendPlan {                   // what the deciding workgroup leaves for the launch that writes
   int32_t *begin, *source;            // [B]: position of the first token (-1: nothing to write); page whose first tokens are copied or -1
-  int32_t *entry, *fresh;             // pages touched: held page + 1 | TAKE; free pages taken
+  int32_t *give_from, *give_to;       // [B]: places in the sequence's row of the table whose pages are given up
+  int32_t *entry, *fresh;             // pages written to: held page + 1 | TAKE; free pages taken
 };
 constexpr unsigned TAKE = 0x80000000u;
 
-__global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c, const CacheAppend a, const AppendPlan plan) {
-  __shared__ int scratch[17];
-  __shared__ int seq[PLAN], first[PLAN], off[PLAN + 1], taken[PLAN], bad_row[PLAN];
+// T threads: as many as the call has rows, at least, and pages to take, up to 1024 (one wavefront, which needs no barriers, for the steps of up to
+// 64 sequences: 3.7 us where 1024 threads took 9.4)
+template <int T>
+__global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, const CacheAppend a, const AppendPlan plan) {
+  __shared__ int scratch[T / 64];
+  __shared__ int seq[T], first[T], off[T + 1], taken[T], bad_row[T];
   __shared__ int lowest;
   const int b = threadIdx.x;
   int at = 0, count = 0, old = 0, s = -1, last = 0, held = 0, entries = 0;
@@ -67,17 +79,17 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
     if (refused) report(c.status, STATUS_ROW);
     else {
       last = pages_of(at + count); held = pages_of(old);
-      entries = max(last, held) - at / PAGE;
+      entries = count > 0 ? last - at / PAGE : 0;
     }
   }
   first[b] = at / PAGE;
   int total_entries;
-  off[b] = block_scan(refused ? 0 : entries, scratch, total_entries);
-  if (b == PLAN - 1) off[PLAN] = total_entries;
+  off[b] = block_scan<T>(refused ? 0 : entries, scratch, total_entries);
+  if (b == T - 1) off[T] = total_entries;
   __syncthreads();
   // row of an entry: the last one that begins at or in front of it (rows without entries begin where the next one does)
   auto row_of = [&](int e) {
-    int lo = 0, hi = PLAN;
+    int lo = 0, hi = T;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (off[mid] <= e) lo = mid; else hi = mid;
@@ -85,19 +97,18 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
     return lo;
   };
   // what each row needs is kept in its thread's registers: others ask for it through LDS
-  __shared__ int r_at[PLAN], r_last[PLAN], r_held[PLAN], r_count[PLAN];
-  r_at[b] = at; r_last[b] = last; r_held[b] = held; r_count[b] = count;
+  __shared__ int r_at[T], r_held[T];
+  r_at[b] = at; r_held[b] = held;
   __syncthreads();
-  // 1. the pages that the rows touch, and which of them need another
-  for (int e = threadIdx.x; e < total_entries; e += PLAN) {
+  // 1. the pages that the rows write to, and which of them need another
+  for (int e = threadIdx.x; e < total_entries; e += T) {
     const int r = row_of(e), j = first[r] + e - off[r];
     int page = -1;
     if (j < r_held[r]) {
       page = c.page_table[(int64_t)seq[r] * c.max_pages + j];
       if (page < 0 || page >= c.pages) { bad_row[r] = 1; page = -1; }
     }
-    const bool written = j < r_last[r] && r_count[r] > 0;
-    const bool take = written && (page < 0 || c.refs[page] > 1);
+    const bool take = page < 0 || c.refs[page] > 1;
     if (take) atomicAdd(&taken[r], 1);
     plan.entry[e] = (int)((unsigned)(page + 1) | (take ? TAKE : 0u));
   }
@@ -108,26 +119,27 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
     taken[b] = 0;
   }
   int needed;
-  const int rank = block_scan(taken[b], scratch, needed);
+  const int rank = block_scan<T>(taken[b], scratch, needed);
   // 2. free pages, from the lowest number on
   int found = 0;
   const int from = max(0, lowest);
+  constexpr int EACH = 8;              // pages a thread
   if (needed > 0)
-    for (int p0 = from; p0 < c.pages && found < needed; p0 += 4 * PLAN) {
-      int is_free[4], mine = 0;
+    for (int p0 = from; p0 < c.pages && found < needed; p0 += EACH * T) {
+      int is_free[EACH], mine = 0;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int p = p0 + 4 * (int)threadIdx.x + x;
+      for (int x = 0; x < EACH; ++x) {
+        const int p = p0 + EACH * (int)threadIdx.x + x;
         is_free[x] = p < c.pages && c.refs[p] == 0;
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mine += is_free[x];
+      for (int x = 0; x < EACH; ++x) mine += is_free[x];
       int here;
-      int at_rank = found + block_scan(mine, scratch, here);
+      int at_rank = found + block_scan<T>(mine, scratch, here);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < EACH; ++x)
         if (is_free[x]) {
-          if (at_rank < needed) plan.fresh[at_rank] = p0 + 4 * (int)threadIdx.x + x;
+          if (at_rank < needed) plan.fresh[at_rank] = p0 + EACH * (int)threadIdx.x + x;
           ++at_rank;
         }
       found += here;
@@ -137,11 +149,11 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
     report(c.status, STATUS_FULL);
     refused = true;
   }
-  __shared__ int go[PLAN], source[PLAN];
+  __shared__ int go[T], source[T];
   go[b] = b < a.B && !refused;
   source[b] = -1;
   int granted;
-  (void)block_scan(go[b] ? taken[b] : 0, scratch, granted);
+  (void)block_scan<T>(go[b] ? taken[b] : 0, scratch, granted);
   if (threadIdx.x == 0) {
     // pages below the first free one stay used: all free ones in front of the last that is taken are taken
     lowest = granted > 0 ? plan.fresh[granted - 1] + 1 : from;
@@ -149,7 +161,7 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
   __syncthreads();
   // 3. the tables
   int done = 0;
-  for (int e0 = 0; e0 < total_entries; e0 += PLAN) {
+  for (int e0 = 0; e0 < total_entries; e0 += T) {
     const int e = e0 + threadIdx.x;
     int r = -1, page = -1, j = 0;
     bool take = false;
@@ -161,26 +173,24 @@ __global__ __launch_bounds__(PLAN) void append_plan_kernel(const bsattn_cache c,
       take = (x & TAKE) != 0 && !bad_row[r];
     }
     int here;
-    const int k = done + block_scan(take, scratch, here);
+    const int k = done + block_scan<T>(take, scratch, here);
     done += here;
     if (r >= 0 && go[r]) {
-      int32_t* entry = c.page_table + (int64_t)seq[r] * c.max_pages + j;
-      const bool behind = j >= r_last[r];
       if (take) {
         const int taken_page = plan.fresh[k];
-        *entry = taken_page;
+        c.page_table[(int64_t)seq[r] * c.max_pages + j] = taken_page;
         c.refs[taken_page] = 1;
         if (page >= 0 && j == first[r] && r_at[r] % PAGE != 0) source[r] = page;
-      } else if (behind) {
-        *entry = -1;
+        if (page >= 0 && atomicSub(&c.refs[page], 1) == 1) atomicMin(&lowest, page);
       }
-      if ((take || behind) && page >= 0 && atomicSub(&c.refs[page], 1) == 1) atomicMin(&lowest, page);
     }
   }
   __syncthreads();
   if (b < a.B) {
     plan.begin[b] = go[b] && count > 0 ? at : -1;
     plan.source[b] = source[b];
+    plan.give_from[b] = go[b] ? last : 0;
+    plan.give_to[b] = go[b] ? held : 0;
     if (go[b]) c.lengths[s] = at + count;
   }
   if (threadIdx.x == 0) *c.free_from = lowest;
@@ -227,10 +237,15 @@ __global__ __launch_bounds__(256) void append_kernel(const bsattn_cache c, const
   const unsigned bh = blockIdx.x / stretches, stretch = blockIdx.x % stretches;
   const int b = bh / (unsigned)c.heads, h = bh % (unsigned)c.heads;
   const int begin = plan.begin[b];
-  if (begin < 0) return;
   const int s = a.sequences != nullptr ? a.sequences[b] : b, count = a.counts != nullptr ? a.counts[b] : a.N;
-  const int32_t* table = c.page_table + (int64_t)s * c.max_pages;
   const bool values = blockIdx.y != 0;
+  if (stretch == 0 && h == 0 && !values) {
+    // pages behind the new end
+    const int to = plan.give_to[b];
+    for (int j = plan.give_from[b] + threadIdx.x; j < to; j += blockDim.x) give_up(c, c.page_table + (int64_t)s * c.max_pages + j);
+  }
+  if (begin < 0) return;
+  const int32_t* table = c.page_table + (int64_t)s * c.max_pages;
   uint8_t* const codes = values ? c.v_codes : c.k_codes;
   uint8_t* const scales = values ? c.v_scales : c.k_scales;
   if (stretch == 0) {
@@ -359,12 +374,7 @@ __global__ __launch_bounds__(256) void free_kernel(const bsattn_cache c, const i
   const int length = length_of(c, s);
   if (kept >= length) return;
   int32_t* table = c.page_table + (int64_t)s * c.max_pages;
-  for (int j = pages_of(kept) + threadIdx.x; j < pages_of(length); j += 256) {
-    const int page = table[j];
-    table[j] = -1;
-    if (page < 0 || page >= c.pages) report(c.status, STATUS_PAGE);
-    else if (atomicSub(&c.refs[page], 1) == 1) atomicMin(c.free_from, page);
-  }
+  for (int j = pages_of(kept) + threadIdx.x; j < pages_of(length); j += 256) give_up(c, table + j);
   __syncthreads();                     // (all threads have seen the length)
   if (threadIdx.x == 0) c.lengths[s] = kept;
 }
@@ -373,10 +383,10 @@ __global__ __launch_bounds__(256) void free_kernel(const bsattn_cache c, const i
 struct CompactPlan { int32_t *count, *used, *holes, *movers, *to; };      // moves; pages in use; targets and sources; new number of a mover
 
 __global__ __launch_bounds__(PLAN) void compact_plan_kernel(const bsattn_cache c, const CompactPlan plan) {
-  __shared__ int scratch[17];
+  __shared__ int scratch[PLAN / 64];
   int used = 0, mine = 0;
   for (int p = threadIdx.x; p < c.pages; p += PLAN) mine += c.refs[p] > 0;
-  (void)block_scan(mine, scratch, used);
+  (void)block_scan<PLAN>(mine, scratch, used);
   int holes = 0, movers = 0;
   for (int p0 = 0; p0 < c.pages; p0 += 4 * PLAN) {
     int refs[4], x_holes = 0, x_movers = 0;
@@ -388,7 +398,7 @@ __global__ __launch_bounds__(PLAN) void compact_plan_kernel(const bsattn_cache c
       x_movers += p >= used && refs[x] > 0;
     }
     int n_holes, n_movers;
-    int at_hole = holes + block_scan(x_holes, scratch, n_holes), at_mover = movers + block_scan(x_movers, scratch, n_movers);
+    int at_hole = holes + block_scan<PLAN>(x_holes, scratch, n_holes), at_mover = movers + block_scan<PLAN>(x_movers, scratch, n_movers);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int p = p0 + 4 * (int)threadIdx.x + x;
@@ -449,14 +459,10 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const bsattn_cache c,
 // ---- host ----
 static size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
-// Entries of the tables that an append may look at: the pages that a row writes to and those behind them
-static int64_t append_entries(const bsattn_cache& c, int B) { return (int64_t)B * c.max_pages; }
-static int64_t append_pages(const bsattn_cache& c, int B, int N) {
-  const int64_t n = (int64_t)B * (N / PAGE + 2);
-  return n < c.pages ? n : c.pages;
-}
-size_t cache_append_workspace_bytes(const bsattn_cache& c, int B, int N) {
-  return 2 * rounded((size_t)B * 4) + rounded((size_t)append_entries(c, B) * 4) + rounded((size_t)append_pages(c, B, N) * 4);
+// Pages that an append of B rows of N tokens may write to
+static int64_t append_pages(int B, int N) { return (int64_t)B * (N / PAGE + 2); }
+size_t cache_append_workspace_bytes(int B, int N) {
+  return 4 * rounded((size_t)B * 4) + 2 * rounded((size_t)append_pages(B, N) * 4);
 }
 
 int launch_cache_append(const bsattn_cache& c, const CacheAppend& a, void* ws, hipStream_t st) {
@@ -464,20 +470,23 @@ int launch_cache_append(const bsattn_cache& c, const CacheAppend& a, void* ws, h
   char* at = (char*)ws;
   plan.begin = (int32_t*)at; at += rounded((size_t)a.B * 4);
   plan.source = (int32_t*)at; at += rounded((size_t)a.B * 4);
-  plan.entry = (int32_t*)at; at += rounded((size_t)append_entries(c, a.B) * 4);
+  plan.give_from = (int32_t*)at; at += rounded((size_t)a.B * 4);
+  plan.give_to = (int32_t*)at; at += rounded((size_t)a.B * 4);
+  plan.entry = (int32_t*)at; at += rounded((size_t)append_pages(a.B, a.N) * 4);
   plan.fresh = (int32_t*)at;
   const int64_t lanes = (int64_t)a.N * (c.head_dim / 8);
   const int threads = lanes <= 64 ? 64 : 256;
-  const int64_t stretches = lanes > 0 ? (lanes + threads - 1) / threads : 0, blocks = (int64_t)a.B * c.heads * stretches;
+  const int64_t stretches = std::max<int64_t>(1, (lanes + threads - 1) / threads), blocks = (int64_t)a.B * c.heads * stretches;
   if (blocks > 0x7fffffffLL) return BSATTN_ERR_RANGE;
-  hipLaunchKernelGGL(append_plan_kernel, dim3(1), dim3(PLAN), 0, st, c, a, plan);
-  if (blocks > 0) {
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 2), dim3(threads), 0, st, c, a, plan, (unsigned)stretches); };
-    const bool bf16 = c.dtype == BSATTN_BF16;
-    if (c.head_dim == 64) bf16 ? go(append_kernel<64, true>) : go(append_kernel<64, false>);
-    else if (c.head_dim == 128) bf16 ? go(append_kernel<128, true>) : go(append_kernel<128, false>);
-    else bf16 ? go(append_kernel<256, true>) : go(append_kernel<256, false>);
-  }
+  const int64_t take = append_pages(a.B, a.N);
+  if (take <= 128 && a.B <= 64) hipLaunchKernelGGL(append_plan_kernel<64>, dim3(1), dim3(64), 0, st, c, a, plan);
+  else if (take <= 512 && a.B <= 256) hipLaunchKernelGGL(append_plan_kernel<256>, dim3(1), dim3(256), 0, st, c, a, plan);
+  else hipLaunchKernelGGL(append_plan_kernel<PLAN>, dim3(1), dim3(PLAN), 0, st, c, a, plan);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 2), dim3(threads), 0, st, c, a, plan, (unsigned)stretches); };
+  const bool bf16 = c.dtype == BSATTN_BF16;
+  if (c.head_dim == 64) bf16 ? go(append_kernel<64, true>) : go(append_kernel<64, false>);
+  else if (c.head_dim == 128) bf16 ? go(append_kernel<128, true>) : go(append_kernel<128, false>);
+  else bf16 ? go(append_kernel<256, true>) : go(append_kernel<256, false>);
   return launch_status();
 }
 
