@@ -230,6 +230,10 @@ __device__ __forceinline__ unsigned quantise8(uintx4 x, int& byte) {
   return w;
 }
 
+// What a thread has under way: the data of a page are three loads behind each other (sequence, table, page), 3 us that one 16-byte piece
+// a thread left half of the bandwidth unused for (8 000 tokens of four prompts read back: 40 us, 1 050 MB 397).
+constexpr int AT_ONCE = 4;
+
 // Grid: (rows x heads x stretches of a row's tokens, keys and values).  A lane takes 8 values: 16 bytes in, 4 out.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void append_kernel(const bsattn_cache c, const CacheAppend a, const AppendPlan plan, unsigned stretches) {
@@ -263,18 +267,43 @@ __global__ __launch_bounds__(256) void append_kernel(const bsattn_cache c, const
   const unsigned short* x = (const unsigned short*)(values ? a.v : a.k);
   const int64_t* xs = values ? a.vs : a.ks;
   x += b * xs[0] + h * xs[1];
-  const unsigned i = stretch * blockDim.x + threadIdx.x;
-  const int token = (int)(i / PER), d = (int)(i % PER);
-  if (token >= count) return;                          // (whole groups of four lanes: PER is a multiple of 4)
-  int byte;
-  const unsigned w = quantise8<BF16>(*reinterpret_cast<const uintx4*>(x + token * xs[2] + 8 * d), byte);
-  const int at = begin + token, slot = at % PAGE;
-  const int64_t page = page_of_head(c, table[at / PAGE], h);
-  *reinterpret_cast<unsigned*>(codes + page * page_codes(D) + slot * (D / 2) + 4 * d) = w;
-  if ((d & 3) == 0) scales[page * page_scales(D) + (d >> 2) * PAGE + scale_at(slot)] = (uint8_t)byte;
+  uintx4 in[AT_ONCE];
+  int pages[AT_ONCE];
+#pragma unroll
+  for (int y = 0; y < AT_ONCE; ++y) {
+    const unsigned i = (stretch * AT_ONCE + y) * blockDim.x + threadIdx.x;
+    const int token = min((int)(i / PER), count - 1), d = (int)(i % PER);
+    in[y] = *reinterpret_cast<const uintx4*>(x + token * xs[2] + 8 * d);
+    pages[y] = table[(begin + token) / PAGE];
+  }
+#pragma unroll
+  for (int y = 0; y < AT_ONCE; ++y) {
+    const unsigned i = (stretch * AT_ONCE + y) * blockDim.x + threadIdx.x;
+    const int token = (int)(i / PER), d = (int)(i % PER);
+    if (token >= count) break;                         // (whole groups of four lanes: PER is a multiple of 4)
+    int byte;
+    const unsigned w = quantise8<BF16>(in[y], byte);
+    const int slot = (begin + token) % PAGE;
+    const int64_t page = page_of_head(c, pages[y], h);
+    *reinterpret_cast<unsigned*>(codes + page * page_codes(D) + slot * (D / 2) + 4 * d) = w;
+    if ((d & 3) == 0) scales[page * page_scales(D) + (d >> 2) * PAGE + scale_at(slot)] = (uint8_t)byte;
+  }
 }
 
 // ---- read ----
+template <bool BF16>
+__device__ __forceinline__ uintx4 values8(unsigned w, float scale) {
+  if constexpr (BF16)
+    return uintx4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+  else
+    return uintx4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+}
 struct CacheRead {
   void *k, *v;
   int64_t ks[3], vs[3];
@@ -287,36 +316,44 @@ __global__ __launch_bounds__(256) void read_kernel(const bsattn_cache c, const C
   const unsigned bh = blockIdx.x / stretches, stretch = blockIdx.x % stretches;
   const int b = bh / (unsigned)c.heads, h = bh % (unsigned)c.heads;
   const bool values = blockIdx.y != 0;
-  const unsigned i = stretch * blockDim.x + threadIdx.x;
-  const int token = (int)(i / PER), d = (int)(i % PER);
-  if (token >= a.N) return;
-  const int s = sequence_of(a.sequences, b, c.sequences);
+  const int s = sequence_of(a.sequences, b, c.sequences), length = s >= 0 ? length_of(c, s) : 0;
   if (s < 0) report(c.status, STATUS_ROW);
-  const int64_t at = (int64_t)(a.start != nullptr ? a.start[b] : 0) + token;
-  uintx4 out = {0, 0, 0, 0};
-  if (s >= 0 && at >= 0 && at < length_of(c, s)) {
-    const int page = c.page_table[(int64_t)s * c.max_pages + at / PAGE], slot = (int)(at % PAGE);
-    if (page < 0 || page >= c.pages) report(c.status, STATUS_PAGE);
-    else {
-      const int64_t head = page_of_head(c, page, h);
-      const unsigned w = *reinterpret_cast<const unsigned*>((values ? c.v_codes : c.k_codes) + head * page_codes(D) + slot * (D / 2) + 4 * d);
-      const float scale = __builtin_bit_cast(float, (unsigned)(values ? c.v_scales : c.k_scales)[head * page_scales(D) + (d >> 2) * PAGE + scale_at(slot)] << 23);
-      if constexpr (BF16) {
-        out[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
-        out[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
-        out[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
-        out[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
-      } else {
-        out[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
-        out[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1));
-        out[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2));
-        out[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
-      }
+  const int64_t start = a.start != nullptr ? a.start[b] : 0;
+  const uint8_t* const codes = values ? c.v_codes : c.k_codes;
+  const uint8_t* const scales = values ? c.v_scales : c.k_scales;
+  int pages[AT_ONCE];
+#pragma unroll
+  for (int y = 0; y < AT_ONCE; ++y) {
+    const int64_t at = start + (int)(((stretch * AT_ONCE + y) * blockDim.x + threadIdx.x) / PER);
+    pages[y] = -1;
+    if (at >= 0 && at < length) {
+      pages[y] = c.page_table[(int64_t)s * c.max_pages + at / PAGE];
+      if (pages[y] < 0 || pages[y] >= c.pages) { report(c.status, STATUS_PAGE); pages[y] = -1; }
+    }
+  }
+  unsigned w[AT_ONCE], byte[AT_ONCE];
+#pragma unroll
+  for (int y = 0; y < AT_ONCE; ++y) {
+    const unsigned i = (stretch * AT_ONCE + y) * blockDim.x + threadIdx.x;
+    const int slot = (int)((start + i / PER) % PAGE), d = (int)(i % PER);
+    w[y] = byte[y] = 0;
+    if (pages[y] >= 0) {
+      const int64_t head = page_of_head(c, pages[y], h);
+      w[y] = *reinterpret_cast<const unsigned*>(codes + head * page_codes(D) + slot * (D / 2) + 4 * d);
+      byte[y] = scales[head * page_scales(D) + (d >> 2) * PAGE + scale_at(slot)];
     }
   }
   unsigned short* x = (unsigned short*)(values ? a.v : a.k);
   const int64_t* xs = values ? a.vs : a.ks;
-  *reinterpret_cast<uintx4*>(x + b * xs[0] + h * xs[1] + token * xs[2] + 8 * d) = out;
+  x += b * xs[0] + h * xs[1];
+#pragma unroll
+  for (int y = 0; y < AT_ONCE; ++y) {
+    const unsigned i = (stretch * AT_ONCE + y) * blockDim.x + threadIdx.x;
+    const int token = (int)(i / PER), d = (int)(i % PER);
+    if (token >= a.N) break;
+    // (past the L2: 26 -> 24 us, 314 -> 289)
+    __builtin_nontemporal_store(values8<BF16>(w[y], __builtin_bit_cast(float, byte[y] << 23)), reinterpret_cast<uintx4*>(x + token * xs[2] + 8 * d));
+  }
 }
 
 // ---- fork ----
@@ -476,7 +513,7 @@ int launch_cache_append(const bsattn_cache& c, const CacheAppend& a, void* ws, h
   plan.fresh = (int32_t*)at;
   const int64_t lanes = (int64_t)a.N * (c.head_dim / 8);
   const int threads = lanes <= 64 ? 64 : 256;
-  const int64_t stretches = std::max<int64_t>(1, (lanes + threads - 1) / threads), blocks = (int64_t)a.B * c.heads * stretches;
+  const int64_t stretches = std::max<int64_t>(1, (lanes + AT_ONCE * threads - 1) / (AT_ONCE * threads)), blocks = (int64_t)a.B * c.heads * stretches;
   if (blocks > 0x7fffffffLL) return BSATTN_ERR_RANGE;
   const int64_t take = append_pages(a.B, a.N);
   if (take <= 128 && a.B <= 64) hipLaunchKernelGGL(append_plan_kernel<64>, dim3(1), dim3(64), 0, st, c, a, plan);
@@ -495,7 +532,7 @@ int launch_cache_read(const bsattn_cache& c, void* k, void* v, const int64_t* ks
   CacheRead a = {k, v, {ks[0], ks[1], ks[2]}, {vs[0], vs[1], vs[2]}, sequences, start, B, N};
   const int64_t lanes = (int64_t)N * (c.head_dim / 8);
   const int threads = lanes <= 64 ? 64 : 256;
-  const int64_t stretches = (lanes + threads - 1) / threads, blocks = (int64_t)B * c.heads * stretches;
+  const int64_t stretches = (lanes + AT_ONCE * threads - 1) / (AT_ONCE * threads), blocks = (int64_t)B * c.heads * stretches;
   if (blocks > 0x7fffffffLL) return BSATTN_ERR_RANGE;
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, 2), dim3(threads), 0, st, c, a, (unsigned)stretches); };
   const bool bf16 = c.dtype == BSATTN_BF16;
