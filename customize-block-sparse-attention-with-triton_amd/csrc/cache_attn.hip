@@ -205,7 +205,7 @@ __device__ __forceinline__ void merge(float& top, float& sum, floatx4& x, float 
 }
 
 // Workgroups of a compute unit (and wavefronts of a SIMD): what the registers leave room for
-template <int D, int QT> constexpr int PER_CU = D * QT >= 512 || QT == 4 ? 1 : (QT == 1 && D < 128 ? 3 : 2);
+template <int D, int QT> constexpr int PER_CU = D * QT >= 512 ? 1 : (QT == 1 && D < 128 ? 3 : 2);
 
 template <int D, bool BF16, int QT, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel(const CacheAttnParams prm) {
@@ -667,7 +667,7 @@ struct CachePlan { int qt, tiles, W; int64_t units; };
 static CachePlan cache_plan(const bsattn_cache& c, int B, int H, int N) {
   CachePlan p;
   const int64_t rows = (int64_t)N * (H / c.heads);
-  p.qt = rows <= 16 ? 1 : (rows <= 32 || c.head_dim == 256 ? 2 : 4);
+  p.qt = rows <= 16 ? 1 : 2;
   p.tiles = (int)((rows + 16 * p.qt - 1) / (16 * p.qt));
   p.units = (int64_t)B * p.tiles;
   const int per_cu = p.qt == 1 ? (c.head_dim < 128 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
@@ -701,8 +701,7 @@ static void launch_rows(const CacheAttnParams& prm, unsigned blocks, hipStream_t
 template <int D, bool BF16>
 static void launch_tiles(const CacheAttnParams& prm, int qt, unsigned blocks, hipStream_t st) {
   if (qt == 1) launch_rows<D, BF16, 1>(prm, blocks, st);
-  else if (D == 256 || qt == 2) launch_rows<D, BF16, 2>(prm, blocks, st);
-  else if constexpr (D != 256) launch_rows<D, BF16, 4>(prm, blocks, st);
+  else launch_rows<D, BF16, 2>(prm, blocks, st);
 }
 
 int launch_cache_attn(const bsattn_cache& c, const CacheAttn& a, void* ws, hipStream_t st) {
