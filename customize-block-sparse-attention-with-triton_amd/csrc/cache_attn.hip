@@ -42,7 +42,7 @@ constexpr int STEP = 16;                      // (see above)
 // Pages of the shortest range (parts cost more to merge than pages to walk), and how near to a unit's end a cut goes there.  (Two cuts
 // are always more than NEAR positions apart: one at most is near an end.)
 template <int D, int QT> constexpr int LEAST = QT == 1 && D < 256 ? 8 : (QT == 1 ? 12 : 8);
-constexpr int NEAR = 6, GAP = NEAR + 1;
+constexpr int NEAR = 6, GAP = 12;
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 // Numerators are 2^HEADROOM at most: in fp16, whose steps are equal below 2^-14, small ones keep their digits 15 powers of two further
 // down (without it weights of 2^-16 beside one of 1 were 2^-9 off).
@@ -324,13 +324,15 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     for (int s = 0; s < DT; ++s) o[qt][s] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- the wavefront's positions: from + wave + 4 i, 64 of them looked up at a time ----
-  const int own = to > from + wave ? (to - from - wave + WAVES - 1) / WAVES : 0, columns = unit_positions / STEP;
-  int chunk = -64, table = -1;
+  // ---- the wavefront's pages, 64 positions looked up at a time: every fourth position of the range, or with a mask every fourth kept page
+  // of those that all four wavefronts look up (2 of 200 000 tokens of which a tenth is kept: 25.3 -> 24.4 us)
+  const int own = MASK ? to - from : (to > from + wave ? (to - from - wave + WAVES - 1) / WAVES : 0), columns = unit_positions / STEP;
+  int chunk = -64, table = -1, kept_before = 0;
   unsigned long long bits = 0;
   auto page_at = [&](int i) {                 // page of the wavefront's position i
-    const int x = from + wave + WAVES * i;
-    return MASK ? (x % STEP) * columns + x / STEP : x;
+    if constexpr (!MASK) return from + wave + WAVES * i;
+    const int x = from + i;
+    return (x % STEP) * columns + x / STEP;
   };
   // next kept page: its number in the cache and in the sequence
   auto next = [&](int& page, int& index) -> bool {
@@ -348,6 +350,11 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
             for (int x = 0; x < (by_head ? prm.group : 1); ++x) keep |= tile_mask[x * prm.a.ms[1] + q * prm.a.ms[2] + p * prm.a.ms[3]] != 0;
       if (keep && (table < 0 || table >= c.pages)) { report(c.status, STATUS_PAGE); keep = false; }
       bits = __ballot(keep);
+      if constexpr (MASK) {
+        const int rank = kept_before + __builtin_popcountll(bits & ((1ull << lane) - 1));
+        kept_before += __builtin_popcountll(bits);
+        bits = __ballot(keep && rank % WAVES == wave);
+      }
     }
     const int j = __builtin_ctzll(bits);
     bits &= bits - 1;
@@ -552,9 +559,12 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   bool last_in = true;
   if (splits > 1) {
     // ---- the workgroups meet ----
-    // a workgroup has two parts at most: of the unit that goes on from the range in front of it, and of the one that goes on behind it
-    auto slot_of = [&](int x) { return ((int64_t)(first_wg + x) * 2 + (x == 0)) * late->c.heads + h; };
-    float* slot_o = late->part_o + slot_of(split) * (ROWS * D);
+    // A workgroup has two parts at most: of the unit that goes on from the range in front of it, and of the one that goes on behind it.  Those
+    // of a head lie close together, rows that are not there take no room: what merges them asks many places at once (one sequence of 160 000
+    // tokens, 64 parts a head: with the heads' parts in turn 8.5 us for it, so 5.4).
+    auto slot_of = [&](int x) { return (int64_t)(h * late->W + first_wg + x) * 2 + (x == 0); };
+    const int slot_rows = min(ROWS, late->rows);
+    float* slot_o = late->part_o + slot_of(split) * (slot_rows * D);
     for (int e = threadIdx.x; e < cells; e += 64 * WAVES) {
       const int r = e / QUADS, d = 4 * (e % QUADS);
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
@@ -563,7 +573,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       for (int y = 0; y < WAVES; ++y)
         merge(top, sum, x, lds_ml[2 * (y * real_rows + r)], lds_ml[2 * (y * real_rows + r) + 1], *reinterpret_cast<const floatx4*>(lds + (y * ROWS + r) * PITCH + d));
       coherent_store4(slot_o + 4 * e, x[0], x[1], x[2], x[3]);
-      if (d == 0) coherent_store2(late->part_ml + slot_of(split) * (ROWS * 2) + 2 * r, top, sum);
+      if (d == 0) coherent_store2(late->part_ml + slot_of(split) * (slot_rows * 2) + 2 * r, top, sum);
     }
     wait_vm<0>();
     __syncthreads();
@@ -580,12 +590,9 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     last_in = *lds_last != 0;
     if (last_in) {
       // The parts go to `teams` groups of threads, where there are few rows; the groups meet in LDS
-      const int64_t step = 2 * (int64_t)late->c.heads;                           // slots from part to part, but for the first
       const int teams = max(1, 64 * WAVES / cells);
-      const float* const ml0 = late->part_ml + slot_of(0) * (ROWS * 2);
-      const float* const ml1 = late->part_ml + (slot_of(1) - step) * (ROWS * 2);
-      const float* const o0 = late->part_o + slot_of(0) * (ROWS * D);
-      const float* const o1 = late->part_o + (slot_of(1) - step) * (ROWS * D);
+      const float* const parts_ml = late->part_ml + slot_of(0) * (slot_rows * 2);
+      const float* const parts_o = late->part_o + slot_of(0) * (slot_rows * D);
       // CELLS cells of a thread at a time, and MERGE / CELLS parts of each
       auto add_up = [&](auto count) {
         constexpr int CELLS = decltype(count)::value, PARTS = MERGE / CELLS;
@@ -605,8 +612,9 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
 #pragma unroll
             for (int j = 0; j < PARTS; ++j) {
               const int y = min(y0 + j * teams, splits - 1);
-              const float* at_part = y == 0 ? o0 : o1 + y * step * (ROWS * D);
-              const float* at_ml = y == 0 ? ml0 : ml1 + y * step * (ROWS * 2);
+              const int slot = y == 0 ? 0 : 2 * y - 1;              // (behind the first part's)
+              const float* at_part = parts_o + (int64_t)slot * (slot_rows * D);
+              const float* at_ml = parts_ml + (int64_t)slot * (slot_rows * 2);
 #pragma unroll
               for (int k = 0; k < CELLS; ++k) {
                 ml[j][k] = coherent_load2(at_ml + 2 * (cell[k] / QUADS));
