@@ -39,7 +39,8 @@ int bsattn_cache_append_workspace(const bsattn_cache* cache, int B, int N, size_
   if (const int rc = check_cache(cache); rc != BSATTN_OK) return rc;
   if (bytes == nullptr) return BSATTN_ERR_NULL;
   if (B <= 0 || N < 0) return BSATTN_ERR_SHAPE;
-  if (B > CACHE_ROWS_MAX || N > cache->max_pages * PAGE || (int64_t)B * (N / PAGE + 2) > 0x7fffffffLL) return BSATTN_ERR_RANGE;
+  if (B > CACHE_ROWS_MAX || N > cache->max_pages * PAGE || (int64_t)B * (N / PAGE + 2) > 0x7fffffffLL ||
+      (int64_t)N * (cache->head_dim / 8) > 0x7fffffffLL) return BSATTN_ERR_RANGE;
   *bytes = cache_append_workspace_bytes(B, N);
   return BSATTN_OK;
 }

@@ -384,6 +384,50 @@ def test_long_sequences(dev, D, dtype, heads, group, lengths):
         assert torch.equal(o, o2) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("B,heads,group,D,dtype,most", [(150, 2, 2, 64, F16, 700), (70, 4, 5, 128, BF16, 2000), (520, 8, 1, 64, BF16, 200), (300, 3, 3, 256, F16, 130)])
+def test_many_sequences(dev, B, heads, group, D, dtype, most):
+    """More sequences than a wavefront looks at at a time, than a head has workgroups, and so many that each has a workgroup of its own."""
+    g = torch.Generator().manual_seed(B)
+    lengths = [int(x) for x in torch.exp(torch.rand(B, generator=g) * math.log(most)).long()]
+    lengths[3], lengths[-1] = 0, most
+    cache, ref = make(dev, sum(-(-n // PAGE) for n in lengths) + 2, heads, D, B, most + 4, dtype)
+    k, v = tokens(B, heads, most, D, dtype, g, dev)
+    import fa2_custom_mask as fm
+    fm.cache_append(cache, k, v, counts=ints(lengths, dev))
+    rk, rv = [x.double().cpu().numpy() for x in fm.cache_read(cache, most)]
+    q = torch.randn(B, heads * group, 1, D, generator=g).to(dtype).to(dev)
+    o, lse = fm.cache_attention_lse(q, cache, None, scale_of(D))
+    cache.check()
+    o, lse, q = o.double().cpu().numpy(), lse.double().cpu().numpy(), q.double().cpu().numpy()
+    for b, n in enumerate(lengths):
+        ro, rl, mean = attention(q[b], rk[b, :, :n], rv[b, :, :n], n - 1, scale_of(D))
+        assert within(o[b], ro, mean, dtype), (b, n)
+        assert np.array_equal(lse[b] == -np.inf, rl == -np.inf) and (n == 0 or np.abs(lse[b] - rl).max() <= 2e-4)
+
+
+@pytest.mark.parametrize("heads,group,N,n,D,dtype", [(1, 16, 2200, 2300, 64, F16), (2, 3, 1000, 5000, 128, BF16), (1, 1, 700, 700, 256, F16)])
+def test_long_prompts(dev, heads, group, N, n, D, dtype):
+    """Hundreds of tiles of one sequence, also more than ranges are made for; the masks' rows of 64 queries among them."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(N)
+    cache, ref = make(dev, -(-n // PAGE) + 2, heads, D, 1, n, dtype)
+    k, v = tokens(1, heads, n, D, dtype, g, dev)
+    fm.cache_append(cache, k, v)
+    rk, rv = [x.double()[0] for x in fm.cache_read(cache, n)]
+    q = torch.randn(1, heads * group, N, D, generator=g).to(dtype).to(dev)
+    M = cache.page_table.shape[1]
+    mask = torch.rand(1, heads * group, -(-N // PAGE), M, generator=g).to(dev) < 0.3
+    see = torch.arange(n, device=dev) <= (n - N + torch.arange(N, device=dev))[:, None]
+    for m in (None, mask):
+        o = fm.cache_attention(q, cache, m, scale_of(D))
+        for h in range(heads * group):
+            seen = see if m is None else see & m[0, h].repeat_interleave(PAGE, 0)[:N].repeat_interleave(PAGE, 1)[:, :n]
+            s = (q[0, h].double() @ rk[h // group].T * scale_of(D)).masked_fill(~seen, -math.inf)
+            p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+            assert within(o[0, h], (p @ rv[h // group]).cpu().numpy(), (p @ rv[h // group].abs()).cpu().numpy(), dtype), h
+    cache.check()
+
+
 def test_large_scores(dev):
     """A maximum that grows from page to page, scores that 32 bits of an exponential cannot hold."""
     g = torch.Generator().manual_seed(12)
@@ -656,6 +700,44 @@ def test_captured_steps(dev):
             assert all(torch.equal(a, b) for a, b in zip(back, read))
             assert torch.equal(cache.page_table, eager.page_table) and torch.equal(cache.lengths, eager.lengths)
             cache.check(), eager.check()
+
+
+def test_threads(dev):
+    """Two threads, each with a cache and a stream of its own, and two that share both kinds of calls on one stream."""
+    import threading
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(19)
+    jobs = []
+    for i in range(4):
+        cache, _ = make(dev, 200, 2, 64, 3, 3000, F16)
+        k, v = tokens(3, 2, 1500, 64, F16, g, dev)
+        q = torch.randn(3, 4, 1, 64, generator=g).to(F16).to(dev)
+        jobs.append((cache, k, v, q))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams += [streams[1]] * 2
+    torch.cuda.synchronize()
+    results = [None] * 4
+
+    def work(i):
+        cache, k, v, q = jobs[i]
+        with torch.cuda.stream(streams[i]):
+            for step in range(20):
+                fm.cache_append(cache, k[:, :, step * 70:step * 70 + 70], v[:, :, step * 70:step * 70 + 70])
+                out = fm.cache_attention(q, cache, None, 0.1)
+            results[i] = out
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    for i, (cache, k, v, q) in enumerate(jobs):
+        cache.check()
+        rk, rv = [x.double().cpu().numpy() for x in fm.cache_read(cache, 1400)]
+        want = stands_for(k[:, :, :1400].double().cpu().numpy(), F16)
+        assert np.array_equal(rk, want)
+        for b in range(3):
+            ro, _, mean = attention(q[b].double().cpu().numpy(), rk[b], rv[b], 1399, 0.1)
+            assert within(results[i][b], ro, mean, F16)
 
 
 def test_streams(dev):
