@@ -14,6 +14,18 @@ namespace bsattn {
 
 constexpr int PLAN = 1024;            // threads of a workgroup that decides, at most
 
+// All T threads have come here, and what they wrote into LDS is there.  (One wavefront's accesses to LDS keep their order, and its loads from
+// memory go on.)
+template <int T>
+__device__ __forceinline__ void meet() {
+  if constexpr (T == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
 // Exclusive sum over the workgroup's T threads; total: of all.  scratch: T / 64 words of LDS.
 template <int T>
 __device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
@@ -52,14 +64,41 @@ struct AppendPlan {                   // what the deciding workgroup leaves for 
 };
 constexpr unsigned TAKE = 0x80000000u;
 
-// T threads: as many as the call has rows, at least, and pages to take, up to 1024 (one wavefront, which needs no barriers, for the steps of up to
-// 64 sequences: 3.7 us where 1024 threads took 9.4)
+// Pages that an append of B rows of N tokens may write to
+static int64_t append_pages(int B, int N) { return (int64_t)B * (N / PAGE + 2); }
+
+// T threads: as many as the call has rows, at least, and half the pages that it may write to, up to 1024 (one wavefront, which needs no barriers,
+// for the steps of up to 64 sequences: 4.0 us where 1024 threads took 9.4).  All of its time is loads that wait for each other (row, length, table,
+// holders): the first free pages are looked for beside them, and what it notes for itself stays in LDS where there is room for it.
 template <int T>
 __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, const CacheAppend a, const AppendPlan plan) {
   __shared__ int scratch[T / 64];
-  __shared__ int seq[T], first[T], off[T + 1], taken[T], bad_row[T];
+  __shared__ __align__(16) int seq[T];
+  constexpr int OWNERS = 4096;
+  __shared__ short owner[OWNERS];
+  __shared__ int clash;
+  __shared__ int first[T], off[T + 1], taken[T], bad_row[T];
   __shared__ int lowest;
+  constexpr bool NOTES = T < PLAN;     // at most 2 T pages to write to (launch_cache_append)
+  __shared__ int lds_entry[NOTES ? 2 * T : 1], lds_fresh[NOTES ? 2 * T : 1];
+  int* const entry = NOTES ? lds_entry : plan.entry;
+  int* const fresh = NOTES ? lds_fresh : plan.fresh;
   const int b = threadIdx.x;
+  // how many hold the pages from the first one that may be free on, 4 VECS a thread (the last vector ends with the last page)
+  constexpr int VECS = T == 64 ? 4 : 2, EACH = 4 * VECS;
+  typedef int int4v __attribute__((ext_vector_type(4), aligned(4)));
+  const int from = min(max(0, *c.free_from), c.pages);
+  int4v holders[VECS];
+  auto vec_of = [&](int p0, int x) { return p0 + EACH * (int)threadIdx.x + 4 * x; };
+  auto look = [&](int p0) {
+    if (c.pages >= 4) {
+#pragma unroll
+      for (int x = 0; x < VECS; ++x) holders[x] = *reinterpret_cast<const int4v*>(c.refs + min(vec_of(p0, x), c.pages - 4));
+    } else {
+#pragma unroll
+      for (int x = 0; x < VECS; ++x) holders[x] = int4v{c.refs[0], c.pages > 1 ? c.refs[1] : -1, c.pages > 2 ? c.refs[2] : -1, -1};
+    }
+  };
   int at = 0, count = 0, old = 0, s = -1, last = 0, held = 0, entries = 0;
   if (b < a.B) {
     s = sequence_of(a.sequences, b, c.sequences);
@@ -67,15 +106,24 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
     if (s >= 0) old = length_of(c, s);
     at = a.at != nullptr ? a.at[b] : old;
   }
+  look(from);
   seq[b] = s;
+  if (s >= 0) owner[s % (unsigned)OWNERS] = (short)b;
   taken[b] = 0; bad_row[b] = 0;
-  if (b == 0) lowest = *c.free_from;
-  __syncthreads();
+  if (b == 0) clash = 0;
+  meet<T>();
+  // a row finds another one's number where it has put its own: a sequence named twice, or numbers that share the place
+  if (s >= 0 && owner[s % (unsigned)OWNERS] != b) clash = 1;
+  meet<T>();
   bool refused = false;
   if (b < a.B) {
     refused = s < 0 || count < 0 || count > a.N || at < 0 || at > old || (int64_t)at + count > (int64_t)c.max_pages * PAGE;
-    if (a.sequences != nullptr)
-      for (int x = 0; x < b; ++x) refused |= seq[x] == s;
+    if (clash != 0)
+      for (int x = 0; x < a.B; x += 4) {              // (T is a multiple of 4)
+        const uintx4 y = *reinterpret_cast<const uintx4*>(seq + x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) refused |= x + i < b && (int)y[i] == s;
+      }
     if (refused) report(c.status, STATUS_ROW);
     else {
       last = pages_of(at + count); held = pages_of(old);
@@ -86,7 +134,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   int total_entries;
   off[b] = block_scan<T>(refused ? 0 : entries, scratch, total_entries);
   if (b == T - 1) off[T] = total_entries;
-  __syncthreads();
+  meet<T>();
   // row of an entry: the last one that begins at or in front of it (rows without entries begin where the next one does)
   auto row_of = [&](int e) {
     int lo = 0, hi = T;
@@ -99,7 +147,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   // what each row needs is kept in its thread's registers: others ask for it through LDS
   __shared__ int r_at[T], r_held[T];
   r_at[b] = at; r_held[b] = held;
-  __syncthreads();
+  meet<T>();
   // 1. the pages that the rows write to, and which of them need another
   for (int e = threadIdx.x; e < total_entries; e += T) {
     const int r = row_of(e), j = first[r] + e - off[r];
@@ -110,9 +158,9 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
     }
     const bool take = page < 0 || c.refs[page] > 1;
     if (take) atomicAdd(&taken[r], 1);
-    plan.entry[e] = (int)((unsigned)(page + 1) | (take ? TAKE : 0u));
+    entry[e] = (int)((unsigned)(page + 1) | (take ? TAKE : 0u));
   }
-  __syncthreads();
+  meet<T>();
   if (bad_row[b]) {
     if (!refused) report(c.status, STATUS_PAGE);
     refused = true;
@@ -122,29 +170,22 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   const int rank = block_scan<T>(taken[b], scratch, needed);
   // 2. free pages, from the lowest number on
   int found = 0;
-  const int from = max(0, lowest);
-  constexpr int EACH = 8;              // pages a thread
   if (needed > 0)
     for (int p0 = from; p0 < c.pages && found < needed; p0 += EACH * T) {
-      int is_free[EACH], mine = 0;
+      if (p0 > from) look(p0);
+      unsigned free = 0;
 #pragma unroll
-      for (int x = 0; x < EACH; ++x) {
-        const int p = p0 + EACH * (int)threadIdx.x + x;
-        is_free[x] = p < c.pages && c.refs[p] == 0;
+      for (int x = 0; x < VECS; ++x) {
+        const int at = vec_of(p0, x);
+        const unsigned four = (holders[x][0] == 0 ? 1 : 0) | (holders[x][1] == 0 ? 2 : 0) | (holders[x][2] == 0 ? 4 : 0) | (holders[x][3] == 0 ? 8 : 0);
+        free |= (four >> min(at - min(at, max(0, c.pages - 4)), 4)) << 4 * x;
       }
-#pragma unroll
-      for (int x = 0; x < EACH; ++x) mine += is_free[x];
       int here;
-      int at_rank = found + block_scan<T>(mine, scratch, here);
-#pragma unroll
-      for (int x = 0; x < EACH; ++x)
-        if (is_free[x]) {
-          if (at_rank < needed) plan.fresh[at_rank] = p0 + EACH * (int)threadIdx.x + x;
-          ++at_rank;
-        }
+      int at_rank = found + block_scan<T>(__popc(free), scratch, here);
+      for (; free != 0 && at_rank < needed; free &= free - 1) fresh[at_rank++] = vec_of(p0, 0) + __builtin_ctz(free);
       found += here;
     }
-  __syncthreads();
+  meet<T>();
   if (!refused && taken[b] > 0 && rank + taken[b] > found) {
     report(c.status, STATUS_FULL);
     refused = true;
@@ -156,9 +197,9 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   (void)block_scan<T>(go[b] ? taken[b] : 0, scratch, granted);
   if (threadIdx.x == 0) {
     // pages below the first free one stay used: all free ones in front of the last that is taken are taken
-    lowest = granted > 0 ? plan.fresh[granted - 1] + 1 : from;
+    lowest = granted > 0 ? fresh[granted - 1] + 1 : from;
   }
-  __syncthreads();
+  meet<T>();
   // 3. the tables
   int done = 0;
   for (int e0 = 0; e0 < total_entries; e0 += T) {
@@ -168,7 +209,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
     if (e < total_entries) {
       r = row_of(e);
       j = first[r] + e - off[r];
-      const unsigned x = (unsigned)plan.entry[e];
+      const unsigned x = (unsigned)entry[e];
       page = (int)(x & ~TAKE) - 1;
       take = (x & TAKE) != 0 && !bad_row[r];
     }
@@ -177,7 +218,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
     done += here;
     if (r >= 0 && go[r]) {
       if (take) {
-        const int taken_page = plan.fresh[k];
+        const int taken_page = fresh[k];
         c.page_table[(int64_t)seq[r] * c.max_pages + j] = taken_page;
         c.refs[taken_page] = 1;
         if (page >= 0 && j == first[r] && r_at[r] % PAGE != 0) source[r] = page;
@@ -185,7 +226,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
       }
     }
   }
-  __syncthreads();
+  meet<T>();
   if (b < a.B) {
     plan.begin[b] = go[b] && count > 0 ? at : -1;
     plan.source[b] = source[b];
@@ -359,9 +400,9 @@ __global__ __launch_bounds__(256) void read_kernel(const bsattn_cache c, const C
 // ---- fork ----
 // A workgroup a pair.  Nothing that one pair reads is written by another: a parent is nobody's child, a child has one pair.
 __global__ __launch_bounds__(256) void fork_kernel(const bsattn_cache c, const int32_t* parents, const int32_t* children, int n) {
-  __shared__ int wrong;
+  __shared__ int wrong, no_page;
   const int i = blockIdx.x, parent = sequence_of(parents, i, c.sequences), child = sequence_of(children, i, c.sequences);
-  if (threadIdx.x == 0) wrong = parent < 0 || child < 0;
+  if (threadIdx.x == 0) { wrong = parent < 0 || child < 0; no_page = 0; }
   __syncthreads();
   for (int x = threadIdx.x; x < n; x += 256) {
     const int y = children[x];
@@ -378,10 +419,10 @@ __global__ __launch_bounds__(256) void fork_kernel(const bsattn_cache c, const i
   int32_t* to = c.page_table + (int64_t)child * c.max_pages;
   for (int j = threadIdx.x; j < pages; j += 256) {
     const int page = from[j];
-    if (page < 0 || page >= c.pages) wrong = 1;
+    if (page < 0 || page >= c.pages) no_page = 1;
   }
   __syncthreads();
-  if (wrong != 0) {
+  if (no_page != 0) {
     if (threadIdx.x == 0) report(c.status, STATUS_PAGE);
     return;
   }
@@ -496,8 +537,6 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const bsattn_cache c,
 // ---- host ----
 static size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
-// Pages that an append of B rows of N tokens may write to
-static int64_t append_pages(int B, int N) { return (int64_t)B * (N / PAGE + 2); }
 size_t cache_append_workspace_bytes(int B, int N) {
   return 4 * rounded((size_t)B * 4) + 2 * rounded((size_t)append_pages(B, N) * 4);
 }

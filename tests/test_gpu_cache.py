@@ -498,6 +498,26 @@ def test_pages_that_do_not_exist(dev):
     said(cache, {2})
 
 
+@pytest.mark.parametrize("rows,sequences", [(3, 4200), (64, 4200), (70, 90), (256, 9000), (300, 9000), (1024, 5000)])
+def test_rows_that_name_a_sequence_twice(dev, rows, sequences):
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(16)
+    cache, ref = make(dev, 1200, 1, 64, sequences, 64, F16)
+    for _ in range(3):                        # the first row of a sequence stands, however far the second is from it
+        named = torch.randperm(sequences, generator=g)[:rows].tolist()
+        if sequences > 4096:
+            named[rows // 2] = (named[0] + 4096) % 8192 if (named[0] + 4096) % 8192 < sequences else named[0] % 100
+        again = named[:-1] + [named[0]]
+        assert append(cache, ref, *tokens(rows, 1, 2, 64, F16, g, dev), sequences=again) == {0}
+        said(cache, {0})
+        same_tables(cache, ref)
+        words = append(cache, ref, *tokens(rows, 1, 2, 64, F16, g, dev), sequences=list(reversed(named)))
+        said(cache, words)
+        same_tables(cache, ref)
+        fm.cache_free(cache)
+        ref.free(range(sequences))
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
