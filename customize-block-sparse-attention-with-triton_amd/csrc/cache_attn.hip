@@ -66,6 +66,17 @@ __device__ __forceinline__ floatx2 coherent_load2(const float* p) {
   return __builtin_bit_cast(floatx2, __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
+// Sixteen, by a buffer's descriptor: of all loads that the compiler waits for by itself only these take 16 bytes past the caches (64 parts in
+// two loads of 8 bytes each: 2.8 us more)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t coherent_memory(float* p, int bytes) {
+  constexpr int WORDS = 0x20000;              // data format: 32 bits
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, WORDS);
+}
+__device__ __forceinline__ floatx4 coherent_load4(__amdgpu_buffer_rsrc_t r, int at) {
+  constexpr int SC1 = 16;
+  return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, SC1));
+}
+
 // row / group, exact for row * group < 2^32
 __device__ __forceinline__ int by_group(unsigned row, int group, unsigned per_group) { return group == 1 ? (int)row : (int)__umulhi(row, per_group); }
 
@@ -276,10 +287,6 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   const int splits = last_wg - first_wg + 1, split = w - first_wg;
   const int from = split == 0 ? 0 : cut_at(w) - unit_begin, to = w == last_wg ? unit_positions : cut_at(w + 1) - unit_begin;      // its positions
 
-  // ---- queries: B operands, lane (n, g) has columns g D / 4 + 8 s .. + 7 of row n ----
-  uintx4 qf[QT][KSTEPS];
-  int limit[QT];                              // last token that the lane's query sees
-  const uint8_t* mrow[QT];                    // its row of the mask
   const bool by_head = MASK && prm.a.mask_heads == 2;
   int block0 = 0, block1 = 0;                 // rows of the mask that the tile's queries have
   const uint8_t* tile_mask = nullptr;         // the first of them, of the tile's first head
@@ -291,6 +298,33 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     tile_mask = prm.a.mask + b * prm.a.ms[0] + (by_head ? h * prm.group : (prm.a.mask_heads == 1 ? h : 0)) * prm.a.ms[1] + block0 * prm.a.ms[2];
   }
   const bool rows_differ = MASK && (by_head || block0 < block1);
+
+  // ---- the wavefront's pages, 64 positions looked up at a time: every fourth position of the range, or with a mask every fourth kept page
+  // of those that all four wavefronts look up (2 of 200 000 tokens of which a tenth is kept: 25.3 -> 24.4 us)
+  const int own = MASK ? to - from : (to > from + wave ? (to - from - wave + WAVES - 1) / WAVES : 0), columns = unit_positions / STEP;
+  auto page_at = [&](int i) {                 // page of the wavefront's position i
+    if constexpr (!MASK) return from + wave + WAVES * i;
+    const int x = from + i;
+    return (x % STEP) * columns + x / STEP;
+  };
+  // the next 64 are asked for when the ones in front of them are taken up, the first ones in front of the queries
+  int chunk = -64, table = -1, kept_before = 0, table_ahead = -1;
+  unsigned char kept_ahead = 0;               // the first of the mask's rows
+  unsigned long long bits = 0;
+  auto ask = [&](int at) {
+    const int p = page_at(at + lane);
+    table_ahead = -1;
+    if (at + lane < own && p < un.pages) {
+      table_ahead = c.page_table[(int64_t)un.seq * c.max_pages + p];
+      if constexpr (MASK) kept_ahead = tile_mask[p * prm.a.ms[3]];
+    }
+  };
+  ask(0);
+
+  // ---- queries: B operands, lane (n, g) has columns g D / 4 + 8 s .. + 7 of row n ----
+  uintx4 qf[QT][KSTEPS];
+  int limit[QT];                              // last token that the lane's query sees
+  const uint8_t* mrow[QT];                    // its row of the mask
   // last token that any of the tile's queries sees
   const int last_token = un.first + min(un.count - 1, by_group(min(prm.rows, (tile + 1) * ROWS) - 1, prm.group, prm.per_group));
 #pragma unroll
@@ -324,16 +358,6 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     for (int s = 0; s < DT; ++s) o[qt][s] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- the wavefront's pages, 64 positions looked up at a time: every fourth position of the range, or with a mask every fourth kept page
-  // of those that all four wavefronts look up (2 of 200 000 tokens of which a tenth is kept: 25.3 -> 24.4 us)
-  const int own = MASK ? to - from : (to > from + wave ? (to - from - wave + WAVES - 1) / WAVES : 0), columns = unit_positions / STEP;
-  int chunk = -64, table = -1, kept_before = 0;
-  unsigned long long bits = 0;
-  auto page_at = [&](int i) {                 // page of the wavefront's position i
-    if constexpr (!MASK) return from + wave + WAVES * i;
-    const int x = from + i;
-    return (x % STEP) * columns + x / STEP;
-  };
   // next kept page: its number in the cache and in the sequence
   auto next = [&](int& page, int& index) -> bool {
     while (bits == 0) {
@@ -341,14 +365,16 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       if (chunk >= own) return false;
       const int p = page_at(chunk + lane);
       const bool there = chunk + lane < own && p < un.pages;
-      table = -1;
-      bool keep = there && !MASK;
-      if (there) table = c.page_table[(int64_t)un.seq * c.max_pages + p];
-      if constexpr (MASK)                     // kept by any of the tile's queries
-        if (there)
+      table = table_ahead;
+      bool keep = there;
+      if constexpr (MASK) {                   // kept by any of the tile's queries
+        keep = there && kept_ahead != 0;
+        if (rows_differ && there)
           for (int q = 0; q <= block1 - block0; ++q)
             for (int x = 0; x < (by_head ? prm.group : 1); ++x) keep |= tile_mask[x * prm.a.ms[1] + q * prm.a.ms[2] + p * prm.a.ms[3]] != 0;
+      }
       if (keep && (table < 0 || table >= c.pages)) { report(c.status, STATUS_PAGE); keep = false; }
+      if (chunk + 64 < own) ask(chunk + 64);
       bits = __ballot(keep);
       if constexpr (MASK) {
         const int rank = kept_before + __builtin_popcountll(bits & ((1ull << lane) - 1));
@@ -592,7 +618,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       // The parts go to `teams` groups of threads, where there are few rows; the groups meet in LDS
       const int teams = max(1, 64 * WAVES / cells);
       const float* const parts_ml = late->part_ml + slot_of(0) * (slot_rows * 2);
-      const float* const parts_o = late->part_o + slot_of(0) * (slot_rows * D);
+      const auto parts_o = coherent_memory(late->part_o + slot_of(0) * (slot_rows * D), 4 * (2 * splits - 1) * (slot_rows * D));
       // CELLS cells of a thread at a time, and MERGE / CELLS parts of each
       auto add_up = [&](auto count) {
         constexpr int CELLS = decltype(count)::value, PARTS = MERGE / CELLS;
@@ -608,18 +634,17 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
             top[k] = -INFINITY; sum[k] = 0.f;
           }
           for (int y0 = team; y0 < splits; y0 += teams * PARTS) {
-            floatx2 ml[PARTS][CELLS], x0[PARTS][CELLS], x1[PARTS][CELLS];
+            floatx2 ml[PARTS][CELLS];
+            floatx4 part[PARTS][CELLS];
 #pragma unroll
             for (int j = 0; j < PARTS; ++j) {
               const int y = min(y0 + j * teams, splits - 1);
               const int slot = y == 0 ? 0 : 2 * y - 1;              // (behind the first part's)
-              const float* at_part = parts_o + (int64_t)slot * (slot_rows * D);
               const float* at_ml = parts_ml + (int64_t)slot * (slot_rows * 2);
 #pragma unroll
               for (int k = 0; k < CELLS; ++k) {
                 ml[j][k] = coherent_load2(at_ml + 2 * (cell[k] / QUADS));
-                x0[j][k] = coherent_load2(at_part + 4 * cell[k]);
-                x1[j][k] = coherent_load2(at_part + 4 * cell[k] + 2);
+                part[j][k] = coherent_load4(parts_o, 4 * (slot * (slot_rows * D) + 4 * cell[k]));
               }
             }
 #pragma unroll
@@ -627,7 +652,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
               if (y0 + j * teams < splits)
 #pragma unroll
                 for (int k = 0; k < CELLS; ++k)
-                  merge(top[k], sum[k], x[k], ml[j][k][0], ml[j][k][1], floatx4{x0[j][k][0], x0[j][k][1], x1[j][k][0], x1[j][k][1]});
+                  merge(top[k], sum[k], x[k], ml[j][k][0], ml[j][k][1], part[j][k]);
           }
 #pragma unroll
           for (int k = 0; k < CELLS; ++k) {
