@@ -116,8 +116,9 @@ template <bool BF16>
 __device__ __forceinline__ uintx4 convert8(unsigned w, float scale) {
   return uintx4{convert2<BF16, 0>(w, scale), convert2<BF16, 1>(w, scale), convert2<BF16, 2>(w, scale), convert2<BF16, 3>(w, scale)};
 }
-// Scale byte `at` of w as a power of two (255: infinity, which the conversions take for "not a number")
-__device__ __forceinline__ float scale_of(unsigned w, int at) { return __builtin_bit_cast(float, ((w >> (8 * at)) & 0xffu) << 23); }
+// Scale byte `at` of w where a conversion takes its power of two from: of the operand only the exponent counts (all codes and scales with 200
+// other patterns in the other bits give the same; 255 is "not a number" whatever they are), so the other bytes may stay
+__device__ __forceinline__ float scale_of(unsigned w, int at) { return __builtin_bit_cast(float, at < 3 ? w << (23 - 8 * at) : w >> 1); }
 
 // Over the four lanes of a query: x and the lane's of the other row of 16 in its pair of rows, then of the other pair.  (The parts of a
 // swap are copied out of its result first: a bit cast of a vector's element takes the vector's first one.)
