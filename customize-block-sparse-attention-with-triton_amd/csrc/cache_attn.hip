@@ -13,8 +13,8 @@
 // What bounds it: one token per sequence reads every kept page once: the cache's bytes (32 sequences of up to 64 000 tokens, 949 MB: 174 us,
 // 5.4 of the 5.85 TB/s that plain reads of pages in any order reach), and below some 100 MB the steps that wait for each other (lengths, table,
 // page, parts: 11 us of the 21 for 58 MB).  Prompt pieces have 32 rows a tile; a wavefront's page (D = 128) takes 128 conversions, 64 byte permutes
-// and about 290 other vector instructions beside 64 matrix ones: the vector ALU bounds it (4 096 queries of 60 000 tokens: 956 TFLOP/s, 777 of
-// 12 000 and of 6 000: 741, with more ends of units in it; a large matrix product 1 202).
+// and about 270 other vector instructions beside 64 matrix ones: the vector ALU bounds it (4 096 queries of 60 000 tokens: 956 TFLOP/s, 777 of
+// 12 000 and of 6 000: 757, with more ends of units in it; a large matrix product 1 202).
 // Measured and not kept: tiles of 64 rows (one wavefront a SIMD, nothing beside its waits); pages converted once for four wavefronts of a workgroup,
 // through LDS (877 for 956 TFLOP/s, and parts of four times the rows to merge); the matrix cores' own 4-bit operands for K with Q in two parts of
 // 8 bits (products are added with 11 bits behind the largest one's first: not a sum in 32 bits).
@@ -44,6 +44,7 @@ namespace bsattn {
 constexpr int WAVES = 4;
 constexpr int MERGE = 16;                     // parts that a thread asks for at a time
 constexpr int STEP = 16;                      // (see above)
+constexpr int AT_ONCE = 4;                    // blocks of 64 units looked at at once
 // Pages of the shortest range (parts cost more to merge than pages to walk), and how near to a unit's end a cut goes there.  (Two cuts
 // are always more than NEAR positions apart: one at most is near an end.)
 template <int D, int QT> constexpr int LEAST = QT == 1 && D < 256 ? 8 : (QT == 1 ? 12 : 8);
@@ -188,16 +189,17 @@ __device__ __forceinline__ void load_values(PageRegs<D>& r, const bsattn_cache& 
 
 // What tile `tile` of row b walks: its sequence, the position of the row's first query, and pages 0 .. pages - 1
 struct Unit { int seq, first, count, pages; };
-template <int ROWS>
+template <int ROWS, bool REPORT>
 __device__ __forceinline__ Unit unit_of(const CacheAttnParams& prm, int b, int tile) {
   Unit u = {sequence_of(prm.a.sequences, b, prm.c.sequences), 0, 0, 0};
   u.count = prm.a.counts != nullptr ? prm.a.counts[b] : prm.a.N;
   if (u.seq < 0 || u.count < 0 || u.count > prm.a.N) {
-    report(prm.c.status, STATUS_ROW);
+    if (REPORT) report(prm.c.status, STATUS_ROW);
     u.seq = -1; u.count = 0;
-    return u;
+    if (REPORT) return u;
   }
-  u.first = length_of(prm.c, u.seq) - u.count;
+  // (without reports there are no branches, so that the loads of several units go out together)
+  u.first = length_of(prm.c, REPORT ? u.seq : max(u.seq, 0)) - u.count;
   int t0 = 0, t1 = prm.a.N - 1;
   if (prm.tiles > 1) {
     t0 = by_group(tile * ROWS, prm.group, prm.per_group);
@@ -240,42 +242,60 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   auto positions = [&](int pages) { return MASK ? (pages + STEP - 1) / STEP * STEP : pages; };
 
   // ---- the range ----
-  Unit mine = {-1, 0, 0, 0};                  // a lane's unit of 64, where it begins on the axis, and how much of the axis it has
-  int begin = 0, length = 0, behind = 0, lo = 0, hi = 0, total = 0, each = 1, longer = 0;
-  bool cut = false;                           // is the range known
+  int lo = 0, hi = 0, each = 1, longer = 0;
   auto cut_at = [&](int x) { return each * x + min(x, longer); };            // begin of range x
   // the range that holds a position
   auto holder = [&](int x) {
     const int of_longer = (each + 1) * longer;
     return x < of_longer ? (int)((unsigned)x / (unsigned)(each + 1)) : longer + (int)((unsigned)(x - of_longer) / (unsigned)each);
   };
-
-  for (int base = prm.W > 0 ? 0 : w;;) {      // units base .. base + 63
-  length = 0;
-  const int lane_unit = base + lane;
-  if (prm.W > 0 ? lane_unit < units : lane == 0) {
-    const int tile_back = prm.tiles == 1 ? 0 : by_group(lane_unit, prm.a.B, prm.per_row);
-    mine = unit_of<ROWS>(prm, lane_unit - tile_back * prm.a.B, prm.tiles - 1 - tile_back);
+  // the workgroup's of an axis of `total` positions; false: it has none
+  auto cut = [&](int total) -> bool {
+    hi = total;
+    if (prm.W == 0) return true;
+    const int ranges = min(prm.W, max(units, total / (LEAST<D, QT>)));
+    if (w >= ranges) return false;
+    // the first `longer` ranges are one position longer than `each`
+    each = (unsigned)total / (unsigned)ranges; longer = total - each * ranges;
+    lo = cut_at(w);
+    hi = lo + each + (w < longer ? 1 : 0);
+    return true;
+  };
+  // Units are looked at 64 at a time, a lane each.  Where there are more, every block's share of the axis is added up first, several blocks' loads
+  // under way at once, and then only those that the range meets are looked at.
+  int starts = 0;                             // where a lane's block begins on the axis
+  unsigned long long blocks = 1;
+  if (prm.W > 0 && units > 64) {
+    int share = 0;
+    for (int k = 0; 64 * k < units; k += AT_ONCE) {
+      int length[AT_ONCE];
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        const int u = min(64 * (k + x) + lane, units - 1), tile_back = prm.tiles == 1 ? 0 : by_group(u, prm.a.B, prm.per_row);
+        length[x] = positions(unit_of<ROWS, false>(prm, u - tile_back * prm.a.B, prm.tiles - 1 - tile_back).pages) + GAP;
+      }
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        const int sum = __builtin_amdgcn_readlane(wave_upto(64 * (k + x) + lane < units ? length[x] : 0), 63);
+        if (lane == k + x) share = sum;
+      }
+    }
+    const int upto = wave_upto(share);
+    if (!cut(__builtin_amdgcn_readlane(upto, 63))) return;
+    starts = upto - share;
+    blocks = __ballot(starts < hi && upto > lo);
+  }
+  for (; blocks != 0; blocks &= blocks - 1) {
+  const int block = __builtin_ctzll(blocks), base = prm.W > 0 ? 64 * block : w;
+  Unit mine = {-1, 0, 0, 0};                  // a lane's unit, how much of the axis it has, and where it begins there
+  int length = 0;
+  if (prm.W > 0 ? base + lane < units : lane == 0) {
+    const int tile_back = prm.tiles == 1 ? 0 : by_group(base + lane, prm.a.B, prm.per_row);
+    mine = unit_of<ROWS, true>(prm, base + lane - tile_back * prm.a.B, prm.tiles - 1 - tile_back);
     length = positions(mine.pages) + GAP;
   }
-  const int upto = wave_upto(length);
-  begin = behind + upto - length;
-  behind += __builtin_amdgcn_readlane(upto, 63);
-  if (!cut) {
-    if (prm.W > 0 && base + 64 < units) { base += 64; continue; }
-    total = behind;
-    hi = total;
-    if (prm.W > 0) {
-      const int ranges = min(prm.W, max(units, total / (LEAST<D, QT>)));
-      if (w >= ranges) return;
-      // the first `longer` ranges are one position longer than `each`
-      each = (unsigned)total / (unsigned)ranges; longer = total - each * ranges;
-      lo = each * w + min(w, longer);
-      hi = lo + each + (w < longer ? 1 : 0);
-    }
-    cut = true;
-    if (base > 0 && prm.W > 0) { base = 0; behind = 0; continue; }
-  }
+  const int upto = wave_upto(length), begin = __builtin_amdgcn_readlane(starts, block) + upto - length;
+  if (hi == 0 && !cut(__builtin_amdgcn_readlane(upto, 63))) return;
   for (unsigned long long mates = __ballot(length > 0 && begin < hi && begin + length > lo); mates != 0; mates &= mates - 1) {
   const int at = __builtin_ctzll(mates), unit = base + at, unit_back = prm.tiles == 1 ? 0 : by_group(unit, prm.a.B, prm.per_row);
   const int b = unit - unit_back * prm.a.B, tile = prm.tiles - 1 - unit_back;
@@ -698,8 +718,6 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     }
   __syncthreads();                            // (the next unit's parts go where these are)
   }
-  if (behind >= hi) break;
-  base += 64;
   }
 }
 
@@ -714,8 +732,12 @@ static CachePlan cache_plan(const bsattn_cache& c, int B, int H, int N) {
   p.units = (int64_t)B * p.tiles;
   const int per_cu = p.qt == 1 ? (c.head_dim < 128 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
   const int64_t fill = (int64_t)compute_units() * per_cu;
-  // ranges where a workgroup a unit would leave compute units idle or wait for the longest sequence (the axis is counted in 32 bits)
-  const bool ranges = p.units * c.heads < 4 * fill && p.units <= 1024 && p.units * ((int64_t)c.max_pages + STEP + GAP) < 0x7fffffffLL;
+  // ranges where a workgroup a unit would leave compute units idle or wait for the longest sequence (the axis is counted in 32 bits).  Sequences
+  // of one length do better without sooner, by 5 to 8 %; those of different lengths lose by it: 16 prompts of 1 000 to 9 000 tokens, 300 queries, 9 rounds
+  // of units 411 us in ranges, 491 without; 24 of 200 to 4 000, 5 rounds 81 and 94.  One token of many sequences: 256 of 200 to 16 000, 4 rounds
+  // 190 and 222, the same at 6 rounds; every workgroup looks through the units of its head, 1 000 of which take 53 us where a workgroup each takes 37.
+  const bool pieces = p.tiles > 1;
+  const bool ranges = p.units * c.heads < (pieces ? 16 : 6) * fill && p.units <= (pieces ? 2048 : 512) && p.units * ((int64_t)c.max_pages + STEP + GAP) < 0x7fffffffLL;
   p.W = ranges ? (int)std::max<int64_t>(1, fill / c.heads) : 0;
   return p;
 }

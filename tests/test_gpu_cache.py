@@ -405,6 +405,30 @@ def test_many_sequences(dev, B, heads, group, D, dtype, most):
         assert np.array_equal(lse[b] == -np.inf, rl == -np.inf) and (n == 0 or np.abs(lse[b] - rl).max() <= 2e-4)
 
 
+@pytest.mark.parametrize("B,heads,group,N,D,dtype,most", [(24, 8, 4, 100, 64, F16, 500), (100, 8, 6, 60, 64, BF16, 200), (70, 2, 3, 90, 128, F16, 900), (130, 3, 1, 33, 256, BF16, 300)])
+def test_many_pieces(dev, B, heads, group, N, D, dtype, most):
+    """Pieces of many prompts: units in ranges, more than a wavefront looks at at a time, and so many that each has a workgroup of its own."""
+    g = torch.Generator().manual_seed(B + N)
+    lengths = [max(1, int(x)) for x in torch.exp(torch.rand(B, generator=g) * math.log(most)).long()]
+    lengths[-1] = most
+    counts = [min(N, n) if b % 3 else min(n, 1 + b % N) for b, n in enumerate(lengths)]
+    cache, ref = make(dev, sum(-(-n // PAGE) for n in lengths) + 2, heads, D, B, most + 4, dtype)
+    k, v = tokens(B, heads, most, D, dtype, g, dev)
+    import fa2_custom_mask as fm
+    fm.cache_append(cache, k, v, counts=ints(lengths, dev))
+    rk, rv = [x.double().cpu().numpy() for x in fm.cache_read(cache, most)]
+    q = torch.randn(B, heads * group, N, D, generator=g).to(dtype).to(dev)
+    o, lse = fm.cache_attention_lse(q, cache, None, scale_of(D), counts=ints(counts, dev))
+    cache.check()
+    o, lse, q = o.double().cpu().numpy(), lse.double().cpu().numpy(), q.double().cpu().numpy()
+    for b in list(range(0, B, 7)) + [B - 1]:
+        n, c = lengths[b], counts[b]
+        ro, rl, mean = attention(q[b, :, :c], rk[b, :, :n], rv[b, :, :n], n - c, scale_of(D))
+        assert within(o[b, :, :c], ro, mean, dtype), (b, n, c)
+        assert np.abs(lse[b, :, :c] - rl).max() <= 2e-4
+        assert not o[b, :, c:].any() and (lse[b, :, c:] == -np.inf).all()
+
+
 @pytest.mark.parametrize("heads,group,N,n,D,dtype", [(1, 16, 2200, 2300, 64, F16), (2, 3, 1000, 5000, 128, BF16), (1, 1, 700, 700, 256, F16)])
 def test_long_prompts(dev, heads, group, N, n, D, dtype):
     """Hundreds of tiles of one sequence, also more than ranges are made for; the masks' rows of 64 queries among them."""
