@@ -52,6 +52,17 @@ __device__ __forceinline__ int wave_upto(int x) {
   return x;
 }
 
+// The largest of the wavefront's, none of them negative
+__device__ __forceinline__ int wave_most(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 struct CacheAttn {
   const void* q; void* o; float* lse;
   const uint8_t* mask; int64_t ms[4];                // strides of the mask's batch, heads, blocks of 64 queries, pages (0: one for all)

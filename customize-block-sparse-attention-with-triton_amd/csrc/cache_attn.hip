@@ -249,11 +249,14 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     const int of_longer = (each + 1) * longer;
     return x < of_longer ? (int)((unsigned)x / (unsigned)(each + 1)) : longer + (int)((unsigned)(x - of_longer) / (unsigned)each);
   };
-  // the workgroup's of an axis of `total` positions; false: it has none
-  auto cut = [&](int total) -> bool {
+  // the workgroup's of an axis of `total` positions, of which one unit has `longest`; false: it has none.  What walks a range takes
+  // total / ranges pages' time, what merges the longest unit's parts longest / total * ranges parts' of its rows: their sum is least at MOST ranges.
+  auto cut = [&](int total, int longest) -> bool {
     hi = total;
     if (prm.W == 0) return true;
-    const int ranges = min(prm.W, max(units, total / (LEAST<D, QT>)));
+    constexpr float MOST = 4.3f;
+    const int most = (int)((float)total * MOST * __builtin_amdgcn_rsqf((float)longest * (float)min(ROWS, prm.rows)));
+    const int ranges = min(prm.W, max(units, min(most, total / (LEAST<D, QT>))));
     if (w >= ranges) return false;
     // the first `longer` ranges are one position longer than `each`
     each = (unsigned)total / (unsigned)ranges; longer = total - each * ranges;
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   int starts = 0;                             // where a lane's block begins on the axis
   unsigned long long blocks = 1;
   if (prm.W > 0 && units > 64) {
-    int share = 0;
+    int share = 0, longest = 0;
     for (int k = 0; 64 * k < units; k += AT_ONCE) {
       int length[AT_ONCE];
 #pragma unroll
@@ -278,10 +281,11 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       for (int x = 0; x < AT_ONCE; ++x) {
         const int sum = __builtin_amdgcn_readlane(wave_upto(64 * (k + x) + lane < units ? length[x] : 0), 63);
         if (lane == k + x) share = sum;
+        longest = max(longest, length[x]);
       }
     }
     const int upto = wave_upto(share);
-    if (!cut(__builtin_amdgcn_readlane(upto, 63))) return;
+    if (!cut(__builtin_amdgcn_readlane(upto, 63), wave_most(longest))) return;
     starts = upto - share;
     blocks = __ballot(starts < hi && upto > lo);
   }
@@ -295,7 +299,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
     length = positions(mine.pages) + GAP;
   }
   const int upto = wave_upto(length), begin = __builtin_amdgcn_readlane(starts, block) + upto - length;
-  if (hi == 0 && !cut(__builtin_amdgcn_readlane(upto, 63))) return;
+  if (hi == 0 && !cut(__builtin_amdgcn_readlane(upto, 63), wave_most(length))) return;
   for (unsigned long long mates = __ballot(length > 0 && begin < hi && begin + length > lo); mates != 0; mates &= mates - 1) {
   const int at = __builtin_ctzll(mates), unit = base + at, unit_back = prm.tiles == 1 ? 0 : by_group(unit, prm.a.B, prm.per_row);
   const int b = unit - unit_back * prm.a.B, tile = prm.tiles - 1 - unit_back;
