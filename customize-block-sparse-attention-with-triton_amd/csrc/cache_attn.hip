@@ -10,9 +10,9 @@
 // (D / 8 bytes in a row, 16 rows an instruction), of V for each of its 16 tokens the columns from n D / 16 on (four whole rows an
 // instruction); column block s of the second product is column n D / 16 + s.  The scales lie as the lanes take them (cache.h).
 //
-// What bounds it: one token per sequence reads every kept page once: the cache's bytes (32 sequences of up to 64 000 tokens, 949 MB: 174 us,
-// 5.4 of the 5.85 TB/s that plain reads of pages in any order reach), and below some 100 MB the steps that wait for each other (lengths, table,
-// page, parts: 11 us of the 21 for 58 MB).  Prompt pieces have 32 rows a tile; a wavefront's page (D = 128) takes 128 conversions, 64 byte permutes
+// What bounds it: one token per sequence reads every kept page once: the cache's bytes (32 sequences of up to 64 000 tokens, 949 MB: 172 us,
+// 5.5 of the 5.85 TB/s that plain reads of pages in any order reach), and below some 100 MB the steps that wait for each other (lengths, table,
+// page, parts: 11 us of the 20 for 58 MB).  Prompt pieces have 32 rows a tile; a wavefront's page (D = 128) takes 128 conversions, 64 byte permutes
 // and about 270 other vector instructions beside 64 matrix ones: the vector ALU bounds it (4 096 queries of 60 000 tokens: 956 TFLOP/s, 777 of
 // 12 000 and of 6 000: 757, with more ends of units in it; a large matrix product 1 202).
 // Measured and not kept: tiles of 64 rows (one wavefront a SIMD, nothing beside its waits); pages converted once for four wavefronts of a workgroup,
