@@ -42,7 +42,6 @@
 namespace bsattn {
 
 constexpr int WAVES = 4;
-constexpr int MERGE = 8;                      // parts that a thread asks for at a time (16: more code for the rule of few parts, 24 sequences 20.5 for 19.8 us, 100 parts 1 less)
 constexpr int STEP = 16;                      // (see above)
 constexpr int AT_ONCE = 4;                    // blocks of 64 units looked at at once
 // Pages of the shortest range (parts cost more to merge than pages to walk), and how near to a unit's end a cut goes there.  (Two cuts
@@ -254,7 +253,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
   auto cut = [&](int total, int longest) -> bool {
     hi = total;
     if (prm.W == 0) return true;
-    constexpr float MOST = 4.3f;
+    constexpr float MOST = 4.8f;              // (of 2 to 9, over calls of 1 to 40 rows; 20 sequences of up to 114 000 tokens, 7 tokens of 4 heads on one: 76 us unbounded, so 30)
     const int most = (int)((float)total * MOST * __builtin_amdgcn_rsqf((float)longest * (float)min(ROWS, prm.rows)));
     const int ranges = min(prm.W, max(units, min(most, total / (LEAST<D, QT>))));
     if (w >= ranges) return false;
@@ -652,9 +651,10 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
       const int teams = max(1, 64 * WAVES / cells);
       const float* const parts_ml = late->part_ml + slot_of(0) * (slot_rows * 2);
       const auto parts_o = coherent_memory(late->part_o + slot_of(0) * (slot_rows * D), 4 * (2 * splits - 1) * (slot_rows * D));
-      // CELLS cells of a thread at a time, and MERGE / CELLS parts of each
+      // CELLS cells of a thread at a time, and PARTS parts of each (more of either is more code and more places asked for in vain where there are few
+      // parts, as is the rule: 24 sequences 20.6 us with 16 parts for 20.2, 100 000 tokens of 16 heads on one 36 with four cells for 27)
       auto add_up = [&](auto count) {
-        constexpr int CELLS = decltype(count)::value, PARTS = MERGE / CELLS;
+        constexpr int CELLS = decltype(count)::value, PARTS = CELLS == 1 ? 8 : 6;
         for (int e0 = threadIdx.x; e0 < cells * teams; e0 += 64 * WAVES * CELLS) {
           const int team = e0 / cells;          // (0 where there is more than one cell a thread)
           int cell[CELLS];
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
         }
       };
       if (cells <= 64 * WAVES) add_up(std::integral_constant<int, 1>{});
-      else add_up(std::integral_constant<int, 4>{});
+      else add_up(std::integral_constant<int, 2>{});
       __syncthreads();
       parts_n = teams; part_step = 4 * cells; pitch = D;
       for (int y = threadIdx.x; y < splits; y += 64 * WAVES) __hip_atomic_store(late->flags + slot_of(y), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
