@@ -96,7 +96,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
       for (int x = 0; x < VECS; ++x) holders[x] = *reinterpret_cast<const int4v*>(c.refs + min(vec_of(p0, x), c.pages - 4));
     } else {
 #pragma unroll
-      for (int x = 0; x < VECS; ++x) holders[x] = int4v{c.refs[0], c.pages > 1 ? c.refs[1] : -1, c.pages > 2 ? c.refs[2] : -1, -1};
+      for (int x = 0; x < VECS; ++x) holders[x] = int4v{c.refs[0], c.pages > 1 ? c.refs[1] : 1, c.pages > 2 ? c.refs[2] : 1, 1};
     }
   };
   int at = 0, count = 0, old = 0, s = -1, last = 0, held = 0, entries = 0;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
 #pragma unroll
       for (int x = 0; x < VECS; ++x) {
         const int at = vec_of(p0, x);
-        const unsigned four = (holders[x][0] == 0 ? 1 : 0) | (holders[x][1] == 0 ? 2 : 0) | (holders[x][2] == 0 ? 4 : 0) | (holders[x][3] == 0 ? 8 : 0);
+        const unsigned four = (holders[x][0] <= 0 ? 1 : 0) | (holders[x][1] <= 0 ? 2 : 0) | (holders[x][2] <= 0 ? 4 : 0) | (holders[x][3] <= 0 ? 8 : 0);
         free |= (four >> min(at - min(at, max(0, c.pages - 4)), 4)) << 4 * x;
       }
       int here;
@@ -458,12 +458,15 @@ __global__ __launch_bounds__(256) void free_kernel(const bsattn_cache c, const i
 }
 
 // ---- compact ----
-struct CompactPlan { int32_t *count, *used, *holes, *movers, *to; };      // moves; pages in use; targets and sources; new number of a mover
+struct CompactPlan { int32_t *count, *used, *holes, *movers, *to; };      // moves; pages in use; targets and sources; new number of a page from `used` on
+
+// A page is in use or free, whatever number stands there: so there are as many free ones below `used` as used ones behind, a target for each move.
+__device__ __forceinline__ bool in_use(int refs) { return refs > 0; }
 
 __global__ __launch_bounds__(PLAN) void compact_plan_kernel(const bsattn_cache c, const CompactPlan plan) {
   __shared__ int scratch[PLAN / 64];
   int used = 0, mine = 0;
-  for (int p = threadIdx.x; p < c.pages; p += PLAN) mine += c.refs[p] > 0;
+  for (int p = threadIdx.x; p < c.pages; p += PLAN) mine += in_use(c.refs[p]);
   (void)block_scan<PLAN>(mine, scratch, used);
   int holes = 0, movers = 0;
   for (int p0 = 0; p0 < c.pages; p0 += 4 * PLAN) {
@@ -471,18 +474,18 @@ __global__ __launch_bounds__(PLAN) void compact_plan_kernel(const bsattn_cache c
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int p = p0 + 4 * (int)threadIdx.x + x;
-      refs[x] = p < c.pages ? c.refs[p] : -1;
-      x_holes += p < used && refs[x] == 0;
-      x_movers += p >= used && refs[x] > 0;
+      refs[x] = p < c.pages ? c.refs[p] : 0;
+      x_holes += p < used && !in_use(refs[x]);              // (used <= pages)
+      x_movers += p >= used && in_use(refs[x]);
     }
     int n_holes, n_movers;
     int at_hole = holes + block_scan<PLAN>(x_holes, scratch, n_holes), at_mover = movers + block_scan<PLAN>(x_movers, scratch, n_movers);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int p = p0 + 4 * (int)threadIdx.x + x;
-      if (p < used && refs[x] == 0) plan.holes[at_hole++] = p;
-      if (p >= used && refs[x] > 0) plan.movers[at_mover++] = p;
-      if (p >= used && refs[x] == 0) plan.to[p] = p;
+      if (p < used && !in_use(refs[x])) plan.holes[at_hole++] = p;
+      if (p >= used && in_use(refs[x])) plan.movers[at_mover++] = p;
+      if (p >= used && p < c.pages && !in_use(refs[x])) plan.to[p] = p;
     }
     holes += n_holes; movers += n_movers;
   }

@@ -33,7 +33,7 @@ class PagedCache4:
     k_scales, v_scales  uint8 [pages, heads, head_dim / 32, 4, 4, 4], token t of a page at [t % 4, t // 4 % 4, t // 16]
     page_table          int32 [sequences, pages of one], the pages of a sequence in their order, -1 behind them
     lengths             int32 [sequences]
-    refs                int32 [pages], how many sequences hold a page (0: free)
+    refs                int32 [pages], how many sequences hold a page (0, or less: free)
 
     The tensors may be read at any time; they are written to by the calls below (which keep a note of where free pages begin)."""
 

@@ -399,7 +399,7 @@ typedef struct {
   uint8_t *k_scales, *v_scales; /* [pages, heads, head_dim / 32, 4, 4, 4]: token t at [t % 4, t / 4 % 4, t / 16] */
   int32_t* page_table;          /* [sequences, max_pages]: pages of a sequence in their order, -1 behind them */
   int32_t* lengths;             /* [sequences] tokens */
-  int32_t* refs;                /* [pages] sequences that hold the page, 0: free */
+  int32_t* refs;                /* [pages] sequences that hold the page, 0 (or less): free */
   int32_t* free_from;           /* 1 word: no page below this number is free (0 is always right) */
   int32_t* status;              /* BSATTN_CACHE_STATUS_WORDS words, device or pinned host memory, or NULL */
   int32_t pages, heads, head_dim, sequences, max_pages;

@@ -542,6 +542,35 @@ def test_rows_that_name_a_sequence_twice(dev, rows, sequences):
         ref.free(range(sequences))
 
 
+@pytest.mark.parametrize("pages", [2, 3, 9, 5000])
+def test_holders_below_zero(dev, pages):
+    """Pages whose number of holders is below zero are free: compact has a target for each page it moves, append takes them."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(pages)
+    cache, ref = make(dev, pages, 1, 64, 2, 64 * pages, F16)
+    k, v = tokens(1, 1, 100, 64, F16, g, dev)
+    used = [pages - 1, (pages - 1) // 2]                             # pages of sequence 1, in this order
+    cache.refs[:] = torch.tensor([-1 - p % 3 for p in range(pages)], dtype=torch.int32)
+    cache.refs[used] = 0
+    others = [p for p in range(pages) if p not in used]
+    saved = cache.refs.clone()
+    cache.refs[others] = 1
+    fm.cache_append(cache, k, v, sequences=ints([1], dev))       # (the two pages that are left, lowest number first)
+    assert cache.page_table[1, :2].tolist() == used[::-1]
+    cache.refs.copy_(saved)
+    cache.refs[used] = 1
+    want = [stands_for(x[0].double().cpu().numpy(), F16) for x in (k, v)]
+    fm.cache_compact(cache)
+    assert cache.refs[:2].tolist() == [1, 1] and bool((cache.refs[2:] <= 0).all())
+    assert sorted(cache.page_table[1, :2].tolist()) == [0, 1]
+    for x, y in zip(fm.cache_read(cache, 100, sequences=ints([1], dev)), want):
+        assert np.array_equal(x[0].double().cpu().numpy(), y)
+    if pages > 4:
+        fm.cache_append(cache, *[x[:, :, :70] for x in (k, v)], sequences=ints([0], dev))
+        assert cache.page_table[0, :2].tolist() == [2, 3] and cache.refs[:4].tolist() == [1, 1, 1, 1]
+    cache.check()
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
