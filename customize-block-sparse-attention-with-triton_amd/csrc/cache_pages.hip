@@ -48,12 +48,22 @@ __device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
   return before + upto - x;
 }
 
+// A page loses a holder; whether it was the last one.  A page that nobody holds stays as it is, which is reported (a subtraction that finds no
+// holder left is taken back: until then there is none to be had either, so that as many succeed as there were holders).
+__device__ __forceinline__ bool last_leaves(const bsattn_cache& c, int page) {
+  const int holders = atomicSub(&c.refs[page], 1);
+  if (holders > 0) return holders == 1;
+  atomicAdd(&c.refs[page], 1);
+  report(c.status, STATUS_PAGE);
+  return false;
+}
+
 // An entry of the page table gives its page up
 __device__ __forceinline__ void give_up(const bsattn_cache& c, int32_t* entry) {
   const int page = *entry;
   *entry = -1;
   if (page < 0 || page >= c.pages) report(c.status, STATUS_PAGE);
-  else if (atomicSub(&c.refs[page], 1) == 1) atomicMin(c.free_from, page);
+  else if (last_leaves(c, page)) atomicMin(c.free_from, page);
 }
 
 // ---- append ----
@@ -222,7 +232,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
         c.page_table[(int64_t)seq[r] * c.max_pages + j] = taken_page;
         c.refs[taken_page] = 1;
         if (page >= 0 && j == first[r] && r_at[r] % PAGE != 0) source[r] = page;
-        if (page >= 0 && atomicSub(&c.refs[page], 1) == 1) atomicMin(&lowest, page);
+        if (page >= 0 && last_leaves(c, page)) atomicMin(&lowest, page);
       }
     }
   }

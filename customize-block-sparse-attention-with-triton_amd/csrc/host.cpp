@@ -615,7 +615,7 @@ struct PagedCache : torch::CustomClassHolder {
       throw std::runtime_error("an earlier call on this cache had a row that it refused: a sequence that does not exist or that the call names twice, a position, "
                                "count or keep outside the sequence or its table, or a fork onto a sequence that holds tokens or is a parent");
     if (found == BSATTN_CACHE_FULL) throw std::runtime_error("an earlier append to this cache found no free page: what it was to append is not there");
-    if (found == BSATTN_CACHE_BAD_PAGE) throw std::runtime_error("an earlier call on this cache met a page number in page_table that the cache does not have");
+    if (found == BSATTN_CACHE_BAD_PAGE) throw std::runtime_error("an earlier call on this cache met a page number in page_table that the cache does not have, or a page that it gave up more often than refs says it is held");
   }
 };
 using CachePtr = c10::intrusive_ptr<PagedCache>;

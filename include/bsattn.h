@@ -392,7 +392,8 @@ int bsattn_reorder_inplace(void* const* x, const int64_t* strides, int n, int BS
 #define BSATTN_CACHE_BAD_ROW 0  /* no such sequence, one that an earlier row of the call names too, a position or a count
                                    outside the sequence or its table; fork: a child that holds tokens or is also a parent */
 #define BSATTN_CACHE_FULL 1     /* no free page for what a row appends */
-#define BSATTN_CACHE_BAD_PAGE 2 /* the page table names a page that the cache does not have */
+#define BSATTN_CACHE_BAD_PAGE 2 /* the page table names a page that the cache does not have, or gives up one that has no holder
+                                   left in `refs` (which keeps the number it has) */
 #define BSATTN_CACHE_STATUS_WORDS 3
 typedef struct {
   uint8_t *k_codes, *v_codes;   /* [pages, heads, 64, head_dim / 2]: value 2 i in the lower four bits of byte i */

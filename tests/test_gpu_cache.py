@@ -571,6 +571,39 @@ def test_holders_below_zero(dev, pages):
     cache.check()
 
 
+def test_pages_given_up_more_often_than_held(dev):
+    """Tables that name a page more often than its number of holders says: it is free once, and never held by less than nobody."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(17)
+    cache, _ = make(dev, 8, 1, 64, 6, 256, F16)
+    cache.page_table[:, :2] = ints([[3, 3], [3, 5], [3, 5], [5, 3], [6, 3], [-1, -1]], dev)
+    cache.lengths[:5] = 128
+    cache.refs[:] = ints([0, 0, 0, 2, 0, 4, 0, 0], dev)
+    cache = fm.PagedCache4.of(cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales, cache.page_table, cache.lengths, cache.refs, F16)
+
+    def found(match):
+        with pytest.raises(RuntimeError, match=match):
+            cache.check()
+        cache.check()
+
+    # by a copy on write of three rows, of which the page has two holders
+    fm.cache_append(cache, *tokens(3, 1, 64, 64, F16, g, dev), at=ints([64, 0, 0], dev))
+    found("more often than refs says")
+    assert cache.refs.tolist() == [1, 1, 1, 0, 0, 2, 0, 0] and cache.lengths.tolist() == [128, 64, 64, 128, 128, 0]
+    assert cache.page_table[:3, :2].tolist() == [[3, 0], [1, -1], [2, -1]]
+    # by an append that cuts, and by cache_free
+    fm.cache_append(cache, *tokens(1, 1, 0, 64, F16, g, dev), at=ints([5], dev), sequences=ints([3], dev))
+    found("more often than refs says")
+    assert cache.refs.tolist() == [1, 1, 1, 0, 0, 2, 0, 0] and cache.page_table[3].tolist() == [5, -1, -1, -1]
+    fm.cache_free(cache)
+    found("more often than refs says")
+    assert cache.refs.tolist() == [0, 0, 0, 0, 0, 1, 0, 0] and bool((cache.page_table == -1).all()) and not bool(cache.lengths.any())
+    fm.cache_compact(cache)
+    fm.cache_append(cache, *tokens(1, 1, 200, 64, F16, g, dev))
+    assert cache.refs.tolist() == [1, 1, 1, 1, 1, 0, 0, 0]
+    cache.check()
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
