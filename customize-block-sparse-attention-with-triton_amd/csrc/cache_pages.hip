@@ -68,7 +68,9 @@ __device__ __forceinline__ void give_up(const bsattn_cache& c, int32_t* entry) {
 
 // ---- append ----
 struct AppendPlan {                   // what the deciding workgroup leaves for the launch that writes
-  int32_t *begin, *source;            // [B]: position of the first token (-1: nothing to write); page whose first tokens are copied or -1
+  // [B]: sequence and tokens to write, as the call's numbers had them before it changed anything (they may be the cache's own lengths);
+  // position of the first token (-1: nothing to write); page whose first tokens are copied or -1
+  int32_t *sequence, *count, *begin, *source;
   int32_t *give_from, *give_to;       // [B]: places in the sequence's row of the table whose pages are given up
   int32_t *entry, *fresh;             // pages written to: held page + 1 | TAKE; free pages taken
 };
@@ -238,6 +240,8 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   }
   meet<T>();
   if (b < a.B) {
+    plan.sequence[b] = s;
+    plan.count[b] = count;
     plan.begin[b] = go[b] && count > 0 ? at : -1;
     plan.source[b] = source[b];
     plan.give_from[b] = go[b] ? last : 0;
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(256) void append_kernel(const bsattn_cache c, const
   const unsigned bh = blockIdx.x / stretches, stretch = blockIdx.x % stretches;
   const int b = bh / (unsigned)c.heads, h = bh % (unsigned)c.heads;
   const int begin = plan.begin[b];
-  const int s = a.sequences != nullptr ? a.sequences[b] : b, count = a.counts != nullptr ? a.counts[b] : a.N;
+  const int s = plan.sequence[b], count = plan.count[b];
   const bool values = blockIdx.y != 0;
   if (stretch == 0 && h == 0 && !values) {
     // pages behind the new end
@@ -551,12 +555,14 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const bsattn_cache c,
 static size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t cache_append_workspace_bytes(int B, int N) {
-  return 4 * rounded((size_t)B * 4) + 2 * rounded((size_t)append_pages(B, N) * 4);
+  return 6 * rounded((size_t)B * 4) + 2 * rounded((size_t)append_pages(B, N) * 4);
 }
 
 int launch_cache_append(const bsattn_cache& c, const CacheAppend& a, void* ws, hipStream_t st) {
   AppendPlan plan;
   char* at = (char*)ws;
+  plan.sequence = (int32_t*)at; at += rounded((size_t)a.B * 4);
+  plan.count = (int32_t*)at; at += rounded((size_t)a.B * 4);
   plan.begin = (int32_t*)at; at += rounded((size_t)a.B * 4);
   plan.source = (int32_t*)at; at += rounded((size_t)a.B * 4);
   plan.give_from = (int32_t*)at; at += rounded((size_t)a.B * 4);

@@ -604,6 +604,33 @@ def test_pages_given_up_more_often_than_held(dev):
     cache.check()
 
 
+@pytest.mark.parametrize("rows", [3, 100, 300])
+def test_append_by_the_cache_s_own_numbers(dev, rows):
+    """counts, at and sequences that are the cache's lengths themselves: they count as they were before the call."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(rows)
+    cache, ref = make(dev, 3 * rows, 2, 64, rows, 300, F16)
+    first = [(s + 1) % rows for s in range(rows)] if rows < 64 else [1 + s % 60 for s in range(rows)]
+    assert not append(cache, ref, *tokens(rows, 2, 60, 64, F16, g, dev), counts=first)
+    k, v = tokens(rows, 2, 60, 64, F16, g, dev)
+    fm.cache_append(cache, k, v, counts=cache.lengths)                            # twice as many of each
+    assert not ref.append(k, v, counts=first)
+    same_tables(cache, ref)
+    same_values(cache, ref)
+    fm.cache_append(cache, k[:, :, :7], v[:, :, :7], at=cache.lengths)
+    assert not ref.append(k[:, :, :7], v[:, :, :7], at=list(ref.length))
+    same_tables(cache, ref)
+    same_values(cache, ref)
+    if rows < 64:
+        fm.cache_append(cache, k[:, :, :0], v[:, :, :0], at=ints(first, dev))       # (lengths: a permutation of the sequences)
+        ref.append(k[:, :, :0], v[:, :, :0], at=first)
+        fm.cache_append(cache, k[:, :, :9], v[:, :, :9], sequences=cache.lengths)
+        assert not ref.append(k[:, :, :9], v[:, :, :9], sequences=first)
+        same_tables(cache, ref)
+        same_values(cache, ref)
+    cache.check()
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
