@@ -633,6 +633,19 @@ Tensor row_numbers(const Index& t, const char* name, int64_t rows, const PagedCa
 }
 const int32_t* numbers(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
 
+// Numbers as they are before the call, for launches whose workgroups change the cache's tables while others still read theirs: a copy where
+// they lie in the tables (keep = lengths, say).
+Tensor row_numbers_apart(const Index& t, const char* name, int64_t rows, const PagedCache& cache) {
+  const Tensor x = row_numbers(t, name, rows, cache);
+  if (!x.defined()) return x;
+  const auto* begin = (const char*)x.const_data_ptr();
+  for (const Tensor* y : {&cache.page_table, &cache.lengths, &cache.refs, &cache.free_from}) {
+    const auto* other = (const char*)y->const_data_ptr();
+    if (begin < other + y->nbytes() && other < begin + x.nbytes()) return x.clone();
+  }
+  return x;
+}
+
 void check_tokens(const Tensor& x, const char* name, const PagedCache& cache) {
   if (!x.is_cuda() || x.device() != cache.device()) throw std::runtime_error(std::string(name) + " must live on the cache's GPU (there is no CPU path)");
   if (x.scalar_type() != cache.dtype) throw py::type_error(std::string(name) + " must be of the cache's type");
@@ -724,7 +737,7 @@ void cache_fork(const CachePtr& cache, const Tensor& parents_, const Tensor& chi
   if (parents_.numel() < 1) throw py::value_error("no sequences to fork");
   if (parents_.numel() > cache->c.sequences) throw py::value_error("more children than the cache has sequences");
   c10::DeviceGuard guard(cache->device());
-  const Tensor parents = row_numbers(parents_, "parents", parents_.numel(), *cache), children = row_numbers(children_, "children", parents_.numel(), *cache);
+  const Tensor parents = row_numbers_apart(parents_, "parents", parents_.numel(), *cache), children = row_numbers_apart(children_, "children", parents_.numel(), *cache);
   check(lib.cache_fork(&cache->c, numbers(parents), numbers(children), (int)parents.numel(), stream_of(parents)), "bsattn_cache_fork");
 }
 
@@ -734,7 +747,7 @@ void cache_free(const CachePtr& cache, const Index& sequences_, const Index& kee
   if (n < 1) throw py::value_error("no sequences to free");
   if (n > cache->c.sequences) throw py::value_error("more rows than the cache has sequences");
   c10::DeviceGuard guard(cache->device());
-  const Tensor sequences = row_numbers(sequences_, "sequences", n, *cache), keep = row_numbers(keep_, "keep", n, *cache);
+  const Tensor sequences = row_numbers_apart(sequences_, "sequences", n, *cache), keep = row_numbers_apart(keep_, "keep", n, *cache);
   check(lib.cache_free(&cache->c, numbers(sequences), numbers(keep), (int)n, stream_of(cache->lengths)), "bsattn_cache_free");
 }
 

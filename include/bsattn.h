@@ -437,7 +437,8 @@ int bsattn_cache_attn(const bsattn_cache* cache, const void* q, void* o, float* 
                       const int64_t* q_strides, const int64_t* o_strides, void* workspace, size_t workspace_bytes,
                       void* stream);
 /* children[i], which holds no tokens, becomes a copy of parents[i] that shares its pages (the next append to either copies the
- * page that it writes to).  No sequence may be named twice in children, or in both. */
+ * page that it writes to).  No sequence may be named twice in children, or in both.  (Here and in free the numbers must not lie
+ * in the cache's own arrays: workgroups change these while others still read.) */
 int bsattn_cache_fork(const bsattn_cache* cache, const int32_t* parents, const int32_t* children, int n, void* stream);
 /* Sequences (NULL: the first n) keep their first keep[i] (NULL: 0) tokens and give up the pages behind them; a sequence that
  * has no more than that stays as it is. */

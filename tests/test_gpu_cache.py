@@ -631,6 +631,34 @@ def test_append_by_the_cache_s_own_numbers(dev, rows):
     cache.check()
 
 
+def test_free_and_fork_by_the_cache_s_own_numbers(dev):
+    """keep, sequences, parents and children that are the cache's tables themselves: they count as they were before the call."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(18)
+    S = 2000
+    cache, ref = make(dev, 2 * S, 1, 64, S, 128, F16)
+    for _ in range(5):
+        first = [int(x) for x in torch.randint(1, 129, (1000,), generator=g)]
+        for rows in (list(range(1000)), list(range(1000, S))):
+            assert not append(cache, ref, *tokens(1000, 1, 128, 64, F16, g, dev), counts=first, sequences=rows)
+        order = torch.randperm(S, generator=g).tolist()
+        fm.cache_free(cache, ints(order, dev), keep=cache.lengths)            # sequence order[i] to the length of sequence i
+        assert not ref.free(order, list(ref.length))
+        same_tables(cache, ref)
+        fm.cache_free(cache)
+        ref.free()
+    # lengths that are numbers of sequences: parents 3, 4, 5, and their children 0, 1, 2
+    cache, ref = make(dev, 20, 1, 64, 6, 128, F16)
+    append(cache, ref, *tokens(6, 1, 5, 64, F16, g, dev), counts=[0, 0, 0, 3, 4, 5])
+    fm.cache_fork(cache, cache.lengths[3:], ints([0, 1, 2], dev))
+    assert not ref.fork([3, 4, 5], [0, 1, 2])
+    same_tables(cache, ref)
+    fm.cache_free(cache, cache.lengths[3:], cache.lengths[:3] - 3)
+    assert not ref.free([3, 4, 5], [0, 1, 2])
+    same_tables(cache, ref)
+    cache.check()
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
