@@ -606,16 +606,19 @@ struct PagedCache : torch::CustomClassHolder {
   }
   at::Device device() const { return k_codes.device(); }
 
-  // What calls so far have reported, once
+  // What calls so far have reported, all of it, once
   void poll() {
-    int found = -1;
+    static const char* const what[BSATTN_CACHE_STATUS_WORDS] = {
+        "an earlier call on this cache had a row that it refused: a sequence that does not exist or that the call names twice, a position, "
+        "count or keep outside the sequence or its table, or a fork onto a sequence that holds tokens or is a parent",
+        "an earlier append to this cache found no free page: what it was to append is not there",
+        "an earlier call on this cache met a page number in page_table that the cache does not have, or a page that it gave up more often than refs says it is held"};
+    static_assert(BSATTN_CACHE_BAD_ROW == 0 && BSATTN_CACHE_FULL == 1 && BSATTN_CACHE_BAD_PAGE == 2);
+    std::string found;
     for (int i = 0; i < BSATTN_CACHE_STATUS_WORDS; ++i)
-      if (__atomic_load_n(c.status + i, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(c.status + i, 0, __ATOMIC_RELAXED) != 0 && found < 0) found = i;
-    if (found == BSATTN_CACHE_BAD_ROW)
-      throw std::runtime_error("an earlier call on this cache had a row that it refused: a sequence that does not exist or that the call names twice, a position, "
-                               "count or keep outside the sequence or its table, or a fork onto a sequence that holds tokens or is a parent");
-    if (found == BSATTN_CACHE_FULL) throw std::runtime_error("an earlier append to this cache found no free page: what it was to append is not there");
-    if (found == BSATTN_CACHE_BAD_PAGE) throw std::runtime_error("an earlier call on this cache met a page number in page_table that the cache does not have, or a page that it gave up more often than refs says it is held");
+      if (__atomic_load_n(c.status + i, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(c.status + i, 0, __ATOMIC_RELAXED) != 0)
+        found += (found.empty() ? "" : "; and ") + std::string(what[i]);
+    if (!found.empty()) throw std::runtime_error(found);
   }
 };
 using CachePtr = c10::intrusive_ptr<PagedCache>;

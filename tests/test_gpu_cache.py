@@ -659,6 +659,39 @@ def test_free_and_fork_by_the_cache_s_own_numbers(dev):
     cache.check()
 
 
+def test_every_report_is_told(dev):
+    """Reports of several kinds since the last look are all in the error, each kind once, and in no later one."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(20)
+    texts = ("a row that it refused", "found no free page", "a page number in page_table")
+
+    def told(words):
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError) as e:
+            cache.check()
+        assert [str(e.value).count(x) for x in texts] == [int(w in words) for w in range(3)]
+        cache.check()
+
+    cache, ref = make(dev, 3, 1, 64, 4, 256, F16)
+    k, v = tokens(3, 1, 100, 64, F16, g, dev)
+    assert append(cache, ref, k, v, sequences=[0, 9, 1]) == {0, 1}         # one call: a bad row, and one without pages
+    told({0, 1})
+    same_tables(cache, ref)
+    assert append(cache, ref, k[:1], v[:1], sequences=[2]) == {1}
+    told({1})
+    cache.page_table[0, 1] = 77
+    for twice in range(2):
+        fm.cache_attention(k[:, :, :1], cache, None, 0.1, sequences=ints([0, -1, 1], dev))
+        if twice:
+            told({0, 2})
+        torch.cuda.synchronize()
+        if not twice:
+            with pytest.raises(RuntimeError, match="refused.*page_table"):
+                fm.cache_read(cache, 1)                                    # (any later call tells, and is not made)
+    fm.cache_attention(k[:1, :, :1], cache, None, 0.1)
+    told({2})
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
