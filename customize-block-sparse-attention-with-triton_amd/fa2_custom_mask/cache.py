@@ -6,7 +6,9 @@ the mask of a call chooses pages.  No counterpart in the reference, whose one ca
 
 All bookkeeping (which pages a sequence has, how long it is) is in GPU memory and done by kernels: no call waits for the GPU, and a
 captured step can be replayed while the sequences grow.  What a call finds that it cannot do (no free page, a row that names no
-sequence) it leaves undone and reports: the next call on the cache, or PagedCache4.check(), raises.
+sequence) it leaves undone and reports.  Each later call looks, before it does anything, whether its GPU has reported something by then:
+the first one that finds something raises in place of doing its own work (call it again).  That need not be the very next one, whose look may come
+before the GPU is so far, and the replay of a graph does not look: PagedCache4.check() waits for the GPU and is sure to tell.
 
 `sequences` says which sequence of the cache a row of a call is (default: row b is sequence b); it, `at`, `counts`, `start`, `keep`,
 `parents` and `children` are int32 or int64 tensors on the GPU with one number a row (int32 is taken as it is).
@@ -61,7 +63,7 @@ class PagedCache4:
         self.head_dim, self.dtype, self.device = head_dim, dtype, k_codes.device
 
     def check(self):
-        """Waits for the GPU and raises what the calls so far have reported."""
+        """Waits for the GPU and raises what the calls and replays so far have reported."""
         torch.cuda.synchronize(self.device)
         self._handle.poll()
 
