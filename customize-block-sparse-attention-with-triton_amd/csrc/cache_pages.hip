@@ -180,11 +180,12 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   }
   int needed;
   const int rank = block_scan<T>(taken[b], scratch, needed);
-  // 2. free pages, from the lowest number on
-  int found = 0;
-  if (needed > 0)
-    for (int p0 = from; p0 < c.pages && found < needed; p0 += EACH * T) {
-      if (p0 > from) look(p0);
+  // 2. free pages, from the lowest number on; from page 0 on where there are too few (free_from is a note that may be too high, say of a handle
+  // that has not seen what another one freed: no row is refused for it)
+  int found = 0, start = from;
+  for (bool again = false;; again = true) {
+    for (int p0 = start; p0 < c.pages && found < needed; p0 += EACH * T) {
+      if (again || p0 > from) look(p0);
       unsigned free = 0;
 #pragma unroll
       for (int x = 0; x < VECS; ++x) {
@@ -197,6 +198,9 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
       for (; free != 0 && at_rank < needed; free &= free - 1) fresh[at_rank++] = vec_of(p0, 0) + __builtin_ctz(free);
       found += here;
     }
+    if (found >= needed || start == 0) break;
+    found = 0; start = 0;
+  }
   meet<T>();
   if (!refused && taken[b] > 0 && rank + taken[b] > found) {
     report(c.status, STATUS_FULL);
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(T) void append_plan_kernel(const bsattn_cache c, co
   (void)block_scan<T>(go[b] ? taken[b] : 0, scratch, granted);
   if (threadIdx.x == 0) {
     // pages below the first free one stay used: all free ones in front of the last that is taken are taken
-    lowest = granted > 0 ? fresh[granted - 1] + 1 : from;
+    lowest = granted > 0 ? fresh[granted - 1] + 1 : start;
   }
   meet<T>();
   // 3. the tables

@@ -571,7 +571,7 @@ struct PagedCache : torch::CustomClassHolder {
   at::ScalarType dtype;
 
   PagedCache(const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table, const Tensor& len, const Tensor& ref,
-             int64_t head_dim_, at::ScalarType dtype_)
+             int64_t head_dim_, at::ScalarType dtype_, const std::optional<Tensor>& note)
       : k_codes(kc), k_scales(ks), v_codes(vc), v_scales(vs), page_table(table), lengths(len), refs(ref), head_dim(head_dim_), dtype(dtype_) {
     if (dtype != at::kHalf && dtype != at::kBFloat16) throw py::type_error("a cache is of float16 or bfloat16");
     if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
@@ -592,7 +592,12 @@ struct PagedCache : torch::CustomClassHolder {
     if (kc.numel() == 0 || table.numel() == 0) throw py::value_error("a cache has at least one page, head and sequence");
     for (int64_t n : {kc.size(0), kc.size(1), table.size(0), table.size(1)})
       if (n > INT_MAX) throw py::value_error("a cache's pages, heads and sequences are counted in 32 bits");
-    free_from = at::zeros({1}, ref.options());
+    if (note) {
+      if (!note->is_cuda() || note->device() != kc.device()) throw std::runtime_error("a cache's tensors must all live on one GPU (there is no CPU path)");
+      if (note->scalar_type() != at::kInt) throw py::type_error("free_from must be int32");
+      if (note->dim() != 1 || note->size(0) != 1) throw py::value_error("free_from must be [1]");
+    }
+    free_from = note ? *note : at::zeros({1}, ref.options());
     c.k_codes = (uint8_t*)kc.data_ptr(); c.k_scales = (uint8_t*)ks.data_ptr();
     c.v_codes = (uint8_t*)vc.data_ptr(); c.v_scales = (uint8_t*)vs.data_ptr();
     c.page_table = table.data_ptr<int32_t>(); c.lengths = len.data_ptr<int32_t>(); c.refs = ref.data_ptr<int32_t>();
@@ -795,9 +800,10 @@ PYBIND11_MODULE(_host, m) {
   m.def("cache_compact", &cache_compact);
   py::class_<PagedCache, CachePtr>(m, "PagedCache")
       .def(py::init([](const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table, const Tensor& lengths, const Tensor& refs,
-                       int64_t head_dim, const Tensor& like) {
-        return c10::make_intrusive<PagedCache>(kc, ks, vc, vs, table, lengths, refs, head_dim, like.scalar_type());
+                       int64_t head_dim, const Tensor& like, const std::optional<Tensor>& free_from) {
+        return c10::make_intrusive<PagedCache>(kc, ks, vc, vs, table, lengths, refs, head_dim, like.scalar_type(), free_from);
       }))
+      .def_readonly("free_from", &PagedCache::free_from)
       .def("poll", [](PagedCache& c) { c.poll(); });
   py::class_<TileLists, ListsPtr>(m, "TileLists")
       .def(py::init([](int64_t Bm, int64_t Hm, int64_t nb, py::object device, bool want_groups) {

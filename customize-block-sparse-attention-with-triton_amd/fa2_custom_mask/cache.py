@@ -36,8 +36,11 @@ class PagedCache4:
     page_table          int32 [sequences, pages of one], the pages of a sequence in their order, -1 behind them
     lengths             int32 [sequences]
     refs                int32 [pages], how many sequences hold a page (0, or less: free)
+    free_from           int32 [1], a note of the calls': no page below this number is free
 
-    The tensors may be read at any time; they are written to by the calls below (which keep a note of where free pages begin)."""
+    The tensors may be read at any time, saved, and put back all together; the calls below write to them.  Who frees pages otherwise (by
+    writing to refs) sets free_from to 0, which is always right: where it is too high an append takes free pages of higher numbers than it
+    need, and looks at the lower ones only before it reports that there are none."""
 
     def __init__(self, pages, heads, head_dim, sequences, tokens, dtype=torch.bfloat16, device="cuda"):
         if min(pages, heads, sequences, tokens) < 1:
@@ -49,17 +52,17 @@ class PagedCache4:
                  make(sequences, dtype=torch.int32).zero_(), make(pages, dtype=torch.int32).zero_(), head_dim, dtype)
 
     @classmethod
-    def of(cls, k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, dtype, head_dim=None):
+    def of(cls, k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, dtype, head_dim=None, free_from=None):
         """A cache made of tensors that are there already (not copied; scale bytes at most 140 for float16, 252 for bfloat16, or
-        255)."""
+        255).  free_from: None for a new one that says 0, or that of another cache made of the same tensors."""
         cache = cls.__new__(cls)
-        cache._of(k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, 2 * k_codes.shape[-1] if head_dim is None else head_dim, dtype)
+        cache._of(k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, 2 * k_codes.shape[-1] if head_dim is None else head_dim, dtype, free_from)
         return cache
 
-    def _of(self, k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, head_dim, dtype):
-        self._handle = _host.PagedCache(k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, head_dim, torch.empty(0, dtype=dtype))
+    def _of(self, k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, head_dim, dtype, free_from=None):
+        self._handle = _host.PagedCache(k_codes, k_scales, v_codes, v_scales, page_table, lengths, refs, head_dim, torch.empty(0, dtype=dtype), free_from)
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
-        self.page_table, self.lengths, self.refs = page_table, lengths, refs
+        self.page_table, self.lengths, self.refs, self.free_from = page_table, lengths, refs, self._handle.free_from
         self.head_dim, self.dtype, self.device = head_dim, dtype, k_codes.device
 
     def check(self):

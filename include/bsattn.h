@@ -401,7 +401,9 @@ typedef struct {
   int32_t* page_table;          /* [sequences, max_pages]: pages of a sequence in their order, -1 behind them */
   int32_t* lengths;             /* [sequences] tokens */
   int32_t* refs;                /* [pages] sequences that hold the page, 0 (or less): free */
-  int32_t* free_from;           /* 1 word: no page below this number is free (0 is always right) */
+  int32_t* free_from;           /* 1 word: no page below this number is free (0 is always right; too high, for instance after
+                                   `refs` has been written to: append takes pages from there on first, and the lower ones only
+                                   where these are too few) */
   int32_t* status;              /* BSATTN_CACHE_STATUS_WORDS words, device or pinned host memory, or NULL */
   int32_t pages, heads, head_dim, sequences, max_pages;
   int32_t dtype;                /* BSATTN_F16 or BSATTN_BF16: of what is appended, read back and asked with */
@@ -412,7 +414,7 @@ typedef struct {
  *
  * Append: row b's sequence is cut to its first at[b] tokens (NULL: none are cut) and the first counts[b] (NULL: N) of the N tokens
  * of k, v [B,heads,N,head_dim] go behind them.  Pages: those of the sequence that no other holds are written where they are; where
- * there is none, or others hold it too, the free page of lowest number is taken, in the order of rows and tokens (of a page that
+ * there is none, or others hold it too, the free page of lowest number (from free_from on) is taken, in the order of rows and tokens (of a page that
  * others hold the tokens in front of at[b] are copied into it).  Pages behind the new end are given up.  A row for which there
  * are no pages left is refused, rows behind it that need any too.  k, v: strides in elements of 4 dimensions, innermost 1, rows
  * 16-byte aligned.  Pages given up in a call are free for the next one. */

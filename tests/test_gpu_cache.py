@@ -692,6 +692,83 @@ def test_every_report_is_told(dev):
     told({2})
 
 
+def test_tables_put_back(dev):
+    """The tensors of a cache, saved and put back behind a compaction; appends then take what they took the first time."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(21)
+    cache, ref = make(dev, 40, 1, 64, 5, 640, F16)
+    append(cache, ref, *tokens(5, 1, 300, 64, F16, g, dev))
+    fm.cache_free(cache, ints([0, 2], dev), ints([0, 100], dev))
+    ref.free([0, 2], [0, 100])
+    x = tokens(5, 1, 90, 64, F16, g, dev)
+    state = [cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales, cache.page_table, cache.lengths, cache.refs, cache.free_from]
+    saved = [t.clone() for t in state]
+    fm.cache_append(cache, *x)
+    want = [t.clone() for t in state]
+    for a, b in zip(state, saved):
+        a.copy_(b)
+    fm.cache_compact(cache)
+    assert int(cache.free_from) == 5 * 5 - 5 - 3
+    for a, b in zip(state, saved):
+        a.copy_(b)
+    assert not append(cache, ref, *x)
+    same_tables(cache, ref)
+    same_values(cache, ref)
+    assert all(torch.equal(a, b) for a, b in zip(state[4:], want[4:]))
+    cache.check()
+
+
+def test_free_from_that_is_refused(dev):
+    import fa2_custom_mask as fm
+    a, _ = make(dev, 4, 1, 64, 2, 128, F16)
+    tensors = (a.k_codes, a.k_scales, a.v_codes, a.v_scales, a.page_table, a.lengths, a.refs)
+    for bad, error in ((ints([0, 0], dev), ValueError), (ints([[0]], dev), ValueError), (ints([0], dev, torch.int64), TypeError), (ints([0], "cpu"), RuntimeError)):
+        with pytest.raises(error):
+            fm.PagedCache4.of(*tensors, F16, free_from=bad)
+
+
+@pytest.mark.parametrize("rows,pages", [(1, 7), (1, 3), (1, 6000), (80, 500), (300, 3000)])
+def test_free_from_too_high(dev, rows, pages):
+    """A note of free pages that is too high (refs written to, or pages freed by another handle): free pages from there on come first, then those
+    below; no row is refused for it, and afterwards the note is right again."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(pages)
+    D, M = 64, max(1, pages // rows - 1)
+    a, _ = make(dev, pages, 1, D, rows + 1, M * PAGE, F16)
+    k, v = [x.expand(rows, 1, -1, -1) for x in tokens(1, 1, M * PAGE, D, F16, g, dev)]
+    tensors = (a.k_codes, a.k_scales, a.v_codes, a.v_scales, a.page_table, a.lengths, a.refs)
+    other, shared = fm.PagedCache4.of(*tensors, F16), fm.PagedCache4.of(*tensors, F16, free_from=a.free_from)
+    assert shared.free_from.data_ptr() == a.free_from.data_ptr() and int(other.free_from) == 0
+    fm.cache_append(a, k, v)
+    used = rows * M
+    assert int(a.free_from) == used
+    fm.cache_free(other, ints(list(range(rows)), dev))                     # `a` does not hear of it
+    assert int(a.free_from) == used and int(other.free_from) == 0 and not bool(a.refs.any())
+    fm.cache_append(a, k, v)                                               # (fewer than that many pages are left behind the note)
+    a.check()
+    assert a.page_table[:rows].flatten().tolist() == list(range(used)) and int(a.free_from) == used
+    # enough of them behind the note: these are taken
+    fm.cache_free(shared, ints([0], dev))
+    assert int(a.free_from) == 0
+    a.free_from.fill_(used)
+    fm.cache_append(a, k[:1, :, :1], v[:1, :, :1])
+    a.check()
+    assert int(a.page_table[0, 0]) == used and int(a.free_from) == used + 1
+    # a row that finds too few anywhere is refused; one that does not need more than there are is not
+    some = sorted(torch.randperm(pages, generator=g)[:M - 1].tolist())
+    a.refs.fill_(1)
+    a.refs[some] = 0
+    a.free_from.fill_(some[-1])
+    fm.cache_append(a, k[:1], v[:1], sequences=ints([rows], dev))
+    with pytest.raises(RuntimeError, match="no free page"):
+        a.check()
+    assert int(a.free_from) == 0 and int(a.lengths[rows]) == 0
+    a.free_from.fill_(pages)
+    fm.cache_append(a, k[:1, :, 64:], v[:1, :, 64:], sequences=ints([rows], dev))
+    a.check()
+    assert a.page_table[rows].tolist() == some + [-1] and int(a.free_from) == some[-1] + 1
+
+
 def test_rows_that_are_refused(dev):
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(15)
