@@ -225,7 +225,12 @@ __device__ __forceinline__ void merge(float& top, float& sum, floatx4& x, float 
 // Workgroups of a compute unit (and wavefronts of a SIMD): what the registers leave room for
 template <int D, int QT> constexpr int PER_CU = D * QT >= 512 ? 1 : (QT == 1 && D < 128 ? 3 : 2);
 
-template <int D, bool BF16, int QT, bool MASK>
+// FINE: P goes into the second product as two bf16 parts, the rounded value and what it lacks (2^-17 together), for results in fp32 of a bf16 cache:
+// one part alone leaves them 8 bits behind the point (2e-3 of a result), of which a caller that merges them would get no more than 16-bit results hold.
+// (fp16, which the forward takes for P then, has no room for a cache's values.  An fp16 cache's P has 11 bits already.)  Twice the matrix
+// instructions of the second product: one to five tokens, bound by other things, take 0 to 6 % longer (24 sequences 20.8 -> 21.2 us, 32 long ones 174 both),
+// pieces of prompts up to a quarter (777 tokens of two prompts 228 -> 282, at D = 64 600 of 3 000 to 9 000 54 -> 62).
+template <int D, bool BF16, int QT, bool MASK, bool FINE>
 __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel(const CacheAttnParams prm) {
   constexpr int ROWS = 16 * QT, PITCH = D + 4, KSTEPS = D / 32, DT = D / 16;
   extern __shared__ __align__(16) float lds[];           // [WAVES][ROWS][PITCH] parts of O | their (m, l) | 1 word
@@ -500,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
         }
       odd = __ballot(bad) != 0;
     }
-    uintx4 p[QT][2];
+    uintx4 p[QT][2], rest[QT][2];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       float top = fmaxf(max3f(s[qt][0][0], s[qt][0][1], s[qt][0][2]), s[qt][0][3]);
@@ -526,8 +531,13 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
           l[qt] += e[i];
         }
         // P is rounded to the operands' type: half a step each, without a bias, against sums of the numerators as they are
-        p[qt][t >> 1][2 * (t & 1)] = pack2<BF16>(e[0], e[1]);
-        p[qt][t >> 1][2 * (t & 1) + 1] = pack2<BF16>(e[2], e[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned pair = pack2<BF16>(e[2 * i], e[2 * i + 1]);
+          p[qt][t >> 1][2 * (t & 1) + i] = pair;
+          if constexpr (FINE)
+            rest[qt][t >> 1][2 * (t & 1) + i] = pack2<true>(e[2 * i] - __builtin_bit_cast(float, pair << 16), e[2 * i + 1] - __builtin_bit_cast(float, pair & 0xffff0000u));
+        }
       }
       if (!part || see[qt] >= token0) marks |= 0x10000u << qt;
     }
@@ -559,6 +569,10 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<D, QT>)) void cache_attn_kernel
           for (int qt = 0; qt < QT; ++qt) {
             o[qt][8 * w + 2 * e] = mfma16<BF16>(low, p[qt][half], o[qt][8 * w + 2 * e]);
             o[qt][8 * w + 2 * e + 1] = mfma16<BF16>(high, p[qt][half], o[qt][8 * w + 2 * e + 1]);
+            if constexpr (FINE) {
+              o[qt][8 * w + 2 * e] = mfma16<BF16>(low, rest[qt][half], o[qt][8 * w + 2 * e]);
+              o[qt][8 * w + 2 * e + 1] = mfma16<BF16>(high, rest[qt][half], o[qt][8 * w + 2 * e + 1]);
+            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -754,17 +768,18 @@ size_t cache_attn_workspace_bytes(const bsattn_cache& c, int B, int H, int N) {
   return rounded(slots * rows * c.head_dim * 4) + rounded(slots * rows * 8) + rounded(slots * 8);
 }
 
-template <int D, bool BF16, int QT, bool MASK>
+template <int D, bool BF16, int QT, bool MASK, bool FINE>
 static void launch_one(const CacheAttnParams& prm, unsigned blocks, hipStream_t st) {
   constexpr int LDS = (WAVES * 16 * QT * (D + 4) + ML_FLOATS<D, QT> + 4) * 4;
   static std::atomic<unsigned long long> configured{0};     // raising the dynamic LDS limit is idempotent
-  once_per_device(configured, [] { (void)hipFuncSetAttribute((const void*)cache_attn_kernel<D, BF16, QT, MASK>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
-  hipLaunchKernelGGL((cache_attn_kernel<D, BF16, QT, MASK>), dim3(blocks), dim3(64 * WAVES), LDS, st, prm);
+  once_per_device(configured, [] { (void)hipFuncSetAttribute((const void*)cache_attn_kernel<D, BF16, QT, MASK, FINE>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
+  hipLaunchKernelGGL((cache_attn_kernel<D, BF16, QT, MASK, FINE>), dim3(blocks), dim3(64 * WAVES), LDS, st, prm);
 }
 template <int D, bool BF16, int QT>
 static void launch_rows(const CacheAttnParams& prm, unsigned blocks, hipStream_t st) {
-  if (prm.a.mask != nullptr) launch_one<D, BF16, QT, true>(prm, blocks, st);
-  else launch_one<D, BF16, QT, false>(prm, blocks, st);
+  const bool fine = BF16 && prm.a.out_f32 != 0;
+  if (prm.a.mask != nullptr) fine ? launch_one<D, BF16, QT, true, BF16>(prm, blocks, st) : launch_one<D, BF16, QT, true, false>(prm, blocks, st);
+  else fine ? launch_one<D, BF16, QT, false, BF16>(prm, blocks, st) : launch_one<D, BF16, QT, false, false>(prm, blocks, st);
 }
 template <int D, bool BF16>
 static void launch_tiles(const CacheAttnParams& prm, int qt, unsigned blocks, hipStream_t st) {

@@ -95,7 +95,8 @@ def cache_attention(q, cache, mask, sm_scale, counts=None, sequences=None):
 
 def cache_attention_lse(q, cache, mask, sm_scale, counts=None, sequences=None, out_fp32=False):
     """The same, also returning the natural-log logsumexp [B, H, N] fp32 of the scaled scores seen (-inf: none); out_fp32=True returns o
-    in fp32."""
+    in fp32, for callers that merge it with others' (of a bfloat16 cache it is computed with probabilities of 16 bits behind the point in
+    place of 8)."""
     return _host.cache_attention(cache._handle, q, mask, sm_scale, counts, sequences, out_fp32, True)
 
 

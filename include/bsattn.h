@@ -430,7 +430,9 @@ int bsattn_cache_read(const bsattn_cache* cache, void* k, void* v, const int64_t
  * counts[b] (NULL: N) queries of row b are the last counts[b] tokens of its sequence: query i sits at position
  * lengths - counts[b] + i and sees the tokens up to there.  mask: NULL, or bytes != 0 for the pages that are kept,
  * [1|B, 1|heads|H, 1|ceil(N/64), max_pages], with element strides mask_strides; dimension 2: one row for all queries, or one for
- * each 64 of the call.  o [B,H,N,head_dim] of out_dtype (the cache's or BSATTN_F32), lse fp32 [B,H,N] or NULL, as bsattn_fwd; queries
+ * each 64 of the call.  o [B,H,N,head_dim] of out_dtype (the cache's or BSATTN_F32), lse fp32 [B,H,N] or NULL, as bsattn_fwd.
+ * Probabilities are rounded to the cache's type for the second product (half a step each, as where bsattn_fwd's result is of that
+ * type), with BSATTN_F32 those of a bf16 cache to two bf16 parts together.  Queries
  * that see no token, and those behind counts[b], get O = 0, lse = -inf. */
 int bsattn_cache_attn_workspace(const bsattn_cache* cache, int B, int H, int N, size_t* bytes);
 int bsattn_cache_attn(const bsattn_cache* cache, const void* q, void* o, float* lse, const uint8_t* mask,

@@ -339,6 +339,61 @@ def test_masks(dev, D, dtype, N, group, mask_rows, mask_heads):
     attend(cache, ref, q, mask=wide[..., ::2], counts=[N, max(0, N - 2), N, 0, N])          # strides of its own
 
 
+def close_in_fp32(o, ref, mean):
+    """A result in fp32 of a bf16 cache: half a step of it, P in two bf16 parts (half a step of the second, which is half a step of the first at
+    most: 2^-18 of P, and as much again where it is rounded up to the next power of two), and the sums and exponentials in 32 bits as in
+    within()."""
+    return o.dtype == torch.float32 and bool((np.abs(o.double().cpu().numpy() - ref) <= (2.0 ** -17 + 2.0 ** -12) * mean + 2.0 ** -24 * np.abs(ref) + 2.0 ** -25).all())
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("N,group,masked", [(1, 1, False), (1, 8, True), (5, 3, False), (5, 3, True), (40, 2, False), (70, 1, True)])
+def test_results_in_fp32_of_bf16(dev, D, N, group, masked):
+    """Are not made of probabilities in 8 bits."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(D + N)
+    heads, lengths = 2, [700, 65, N, 333]
+    cache, ref = make(dev, 40, heads, D, 4, 700, BF16)
+    append(cache, ref, *tokens(4, heads, 700, D, BF16, g, dev), counts=lengths)
+    q = torch.randn(4, heads * group, N, D, generator=g).to(BF16).to(dev)
+    mask = (torch.rand(4, heads * group, -(-N // PAGE), 11, generator=g) < 0.6) if masked else None
+    o, _ = attend(cache, ref, q, mask=mask, out_fp32=True)
+    rounded = fm.cache_attention(q, cache, None if mask is None else mask.to(dev), scale_of(D))
+    error, size, coarse = 0.0, 0.0, 0.0
+    for b in range(4):
+        kept = None
+        if masked:
+            kept = mask[b].numpy()[:, [i // PAGE for i in range(N)]]
+        k, v = ref.values(b)
+        ro, _, mean = attention(q[b].double().cpu().numpy(), k, v, lengths[b] - N, scale_of(D), kept)
+        assert close_in_fp32(o[b], ro, mean), b
+        error += ((o[b].double().cpu().numpy() - ro) ** 2).sum()
+        coarse += ((rounded[b].double().cpu().numpy() - ro) ** 2).sum()
+        size += (ro ** 2).sum()
+    assert error <= size * 2.0 ** -28 and error * 100 < coarse            # (2^-14 where the sums of 32 bits do not add up one way)
+
+
+@pytest.mark.parametrize("D,heads,group,N,lengths", [(64, 1, 16, 1, [40000]), (128, 2, 4, 3, [20000, 100, 9000]), (256, 1, 5, 9, [9000, 30])])
+def test_long_results_in_fp32_of_bf16(dev, D, heads, group, N, lengths):
+    """The same where parts of several workgroups are merged."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(D)
+    B = len(lengths)
+    cache, _ = make(dev, sum(-(-n // PAGE) for n in lengths), heads, D, B, max(lengths), BF16)
+    k, v = tokens(B, heads, max(lengths), D, BF16, g, dev)
+    fm.cache_append(cache, k, v, counts=ints(lengths, dev))
+    rk, rv = [x.double().cpu().numpy() for x in fm.cache_read(cache, max(lengths))]
+    q = torch.randn(B, heads * group, N, D, generator=g).to(BF16).to(dev)
+    o, lse = fm.cache_attention_lse(q, cache, None, scale_of(D), out_fp32=True)
+    for b, n in enumerate(lengths):
+        ro, rl, mean = attention(q[b].double().cpu().numpy(), rk[b, :, :n], rv[b, :, :n], n - N, scale_of(D))
+        assert close_in_fp32(o[b], ro, mean), b
+        assert np.abs(lse[b].double().cpu().numpy() - rl).max() <= 2e-4
+    for _ in range(3):
+        assert torch.equal(o, fm.cache_attention_lse(q, cache, None, scale_of(D), out_fp32=True)[0])
+    cache.check()
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
 def test_scales(dev, scale):
     g = torch.Generator().manual_seed(9)
