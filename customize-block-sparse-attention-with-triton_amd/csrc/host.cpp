@@ -195,6 +195,9 @@ ListsPtr block_mask_to_lists(const Tensor& block, bool transpose, bool want_grou
   return lists;
 }
 
+// A dual tensor of forward-mode differentiation whose tangent a call would drop (one that requires no gradient passes all other checks)
+bool has_tangent(const Tensor& x) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined(); }
+
 // ---- q, k, v ----
 void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
   if (!(q.is_cuda() && k.is_cuda() && v.is_cuda())) throw std::runtime_error("q, k, v must be GPU tensors (there is no CPU path)");
@@ -661,6 +664,7 @@ void check_tokens(const Tensor& x, const char* name, const PagedCache& cache) {
   if (x.size(0) < 1) throw py::value_error(std::string(name) + " has no rows");
   if (x.size(0) > INT_MAX || x.size(1) > INT_MAX || x.size(2) > INT_MAX) throw py::value_error(std::string(name) + ": sizes are counted in 32 bits");
   if (at::GradMode::is_enabled() && x.requires_grad()) throw std::runtime_error(std::string(name) + " requires a gradient, and a cache has none: detach it or use torch.no_grad()");
+  if (has_tangent(x)) throw std::runtime_error(std::string(name) + " has a tangent, and a cache has no forward-mode differentiation");
 }
 void check_rows_of(const PagedCache& cache, int64_t rows, const Index& sequences) {
   if (!sequences && rows > cache.c.sequences) throw py::value_error("more rows than the cache has sequences");

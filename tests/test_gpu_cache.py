@@ -917,6 +917,28 @@ def test_refusals(dev):
     cache.check()
 
 
+def test_tangents_are_refused(dev):
+    """A dual tensor that requires no gradient: its tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+    import fa2_custom_mask as fm
+    cache, _ = make(dev, 4, 2, 64, 3, 128, F16)
+    x = torch.ones(1, 2, 5, 64, dtype=F16, device=dev)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: fm.cache_append(cache, dual, x), lambda: fm.cache_append(cache, x, dual), lambda: fm.cache_attention(dual, cache, None, 0.1),
+                     lambda: fm.cache_attention_lse(dual, cache, None, 0.1)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        assert not bool(cache.lengths.any())
+        fm.cache_append(cache, fwad.unpack_dual(dual).primal.detach(), x)
+        with torch.inference_mode():
+            fm.cache_attention(dual, cache, None, 0.1)                     # (nothing is differentiated in there)
+    fm.cache_append(cache, dual, x)                                        # behind its level a dual tensor is none
+    cache.check()
+
+
 # ---- as they are used ----
 def test_far_pages(dev):
     """Codes beyond 4 GB from where they begin."""
