@@ -206,6 +206,7 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
   const auto t = q.scalar_type();
   if ((t != at::kHalf && t != at::kBFloat16) || k.scalar_type() != t || v.scalar_type() != t)
     throw py::type_error("q, k, v must all be float16 or all bfloat16");
+  if (has_tangent(q) || has_tangent(k) || has_tangent(v)) throw std::runtime_error("q, k or v has a tangent: there is no forward-mode differentiation");
   const int64_t D = q.size(3);
   if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256)                       // :58
     throw py::value_error("head dimension must be 16, 32, 64, 128 or 256");

@@ -162,3 +162,25 @@ def test_transforms_are_refused(dev):
     with pytest.raises((RuntimeError, NotImplementedError)):
         with fwad.dual_level():
             fm.flash_attention_custom_mask(fwad.make_dual(q, torch.ones_like(q)), k, v, mask, 0.2)
+
+
+def test_tangents_are_refused_without_gradients(dev):
+    """A dual tensor that requires no gradient: its tangent would be dropped without a word, for a mask that is new and for one that is known."""
+    import fa2_custom_mask as fm
+    import torch.autograd.forward_ad as fwad
+    qkv = [x.to(dev) for x in make_qkv(1, 1, 128, 64, torch.float16, 752)]
+    mask = uniform_block_mask(1, 1, 2, 1.0, 753).to(dev)
+    want = fm.flash_attention_custom_mask(*qkv, mask, 0.2)
+    with fwad.dual_level():
+        for i in range(3):
+            dual = [fwad.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate(qkv)]
+            for m in (mask, mask.clone(), None):
+                with pytest.raises(RuntimeError, match="tangent"):
+                    fm.flash_attention_custom_mask(*dual, m, 0.2)
+                with pytest.raises(RuntimeError, match="tangent"):
+                    fm.flash_attention_custom_mask_lse(*dual, m, 0.2)
+            with pytest.raises(RuntimeError, match="tangent"):
+                fm.attention_forward_backward(*dual, mask, 0.2, want)
+            with torch.inference_mode():
+                assert torch.equal(fm.flash_attention_custom_mask(*dual, mask, 0.2), want)
+    assert torch.equal(fm.flash_attention_custom_mask(*dual, mask, 0.2), want)
