@@ -507,6 +507,115 @@ def test_long_prompts(dev, heads, group, N, n, D, dtype):
     cache.check()
 
 
+# Units with more positions than a wavefront looks up at a time (64 of its own, or with a mask 64 of the workgroup's), in ranges and with a
+# workgroup each: what is asked for ahead, and how many kept pages there were before, go from one round to the next.
+def filled(dev, lengths, heads, D, dtype):
+    """A cache of sequences of these lengths with random codes, scales of 2^-7 .. 2^0, pages in random order."""
+    import fa2_custom_mask as fm
+    count = [-(-n // PAGE) for n in lengths]
+    M = max(count) + 1
+    cache = fm.PagedCache4(sum(count) + 3, heads, D, len(lengths), M * PAGE, dtype, dev)
+    g = torch.Generator(device=dev).manual_seed(sum(count) + D)
+    for x in (cache.k_codes, cache.v_codes):
+        x.random_(0, 256, generator=g)
+    for x in (cache.k_scales, cache.v_scales):
+        x.random_(120, 128, generator=g)
+    order = torch.randperm(sum(count) + 3, generator=g, device=dev, dtype=torch.int32)
+    table, at = torch.full((len(lengths), M), -1, dtype=torch.int32), 0
+    for s, c in enumerate(count):
+        table[s, :c] = order[at:at + c].cpu()
+        at += c
+    cache.page_table.copy_(table)
+    cache.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+    cache.refs[order[:at].long()] = 1
+    return cache, M
+
+
+def agrees(o, lse, q, cache, rows, heads, mask, counts):
+    """These rows and heads of q against 64 bits."""
+    import fa2_custom_mask as fm
+    B, H, N, D = q.shape
+    group, dev = H // cache.k_codes.shape[1], q.device
+    lengths = cache.lengths.tolist()
+    for b in rows:
+        n, c = lengths[b], counts[b]
+        k, v = [x[0] for x in fm.cache_read(cache, n, sequences=ints([b], dev))]
+        behind = torch.arange(n, device=dev) > (n - c + torch.arange(c, device=dev))[:, None]
+        for h in heads:
+            kk, vv = k[h // group].double(), v[h // group].double()
+            s = (q[b, h, :c].double() @ kk.T * scale_of(D)).masked_fill(behind, -math.inf)
+            if mask is not None:
+                m = mask[b % mask.shape[0], h if mask.shape[1] == H else 0]
+                m = m[torch.arange(c, device=dev) // PAGE] if m.shape[0] > 1 else m.expand(c, -1)
+                s = s.masked_fill(~m.repeat_interleave(PAGE, 1)[:, :n], -math.inf)
+            p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+            want = torch.logsumexp(s, -1)
+            assert within(o[b, h, :c], (p @ vv).cpu().numpy(), (p @ vv.abs()).cpu().numpy(), q.dtype), (b, h, n)
+            assert torch.equal(lse[b, h, :c] == -math.inf, want == -math.inf), (b, h)
+            assert bool(((lse[b, h, :c].double() - want).abs() <= 2e-4).logical_or(want == -math.inf).all()), (b, h)
+
+
+def masks_of(g, dev, B, H, rows, M, lengths):
+    """None, one for all heads, and one for each head with heads and stretches that keep nothing."""
+    one = torch.rand(B, 1, rows, M, generator=g) < 0.5
+    each = torch.rand(B, H, rows, M, generator=g) < torch.rand(B, H, rows, 1, generator=g)
+    each[:, 0, :, 64:128] = False
+    each[-1, H - 1] = False
+    thin = torch.zeros(1, 1, 1, M, dtype=torch.bool)
+    thin[..., 70::67] = True
+    return [None] + [m.to(dev) for m in (one, each, thin)]
+
+
+@pytest.mark.parametrize("B,heads,group,D,dtype,longest", [(513, 1, 1, 64, F16, [17000]), (520, 1, 5, 128, BF16, [17100, 36000]), (600, 2, 2, 256, F16, [16500])])
+def test_long_ones_among_many_sequences(dev, B, heads, group, D, dtype, longest):
+    """A workgroup for each sequence, a few of them long."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(B)
+    lengths = [1 + (37 * b) % 100 for b in range(B)]
+    where = [(7 + 255 * i) % B for i in range(len(longest))]
+    for b, n in zip(where, longest):
+        lengths[b] = n
+    cache, M = filled(dev, lengths, heads, D, dtype)
+    q = torch.randn(B, heads * group, 1, D, generator=g).to(dtype).to(dev)
+    for mask in masks_of(g, dev, B, heads * group, 1, M, lengths):
+        o, lse = fm.cache_attention_lse(q, cache, mask, scale_of(D))
+        agrees(o, lse, q, cache, where + [0, 3, B - 1], range(heads * group), mask, [1] * B)
+    cache.check()
+
+
+@pytest.mark.parametrize("heads,group,D,N,dtype,lengths", [(192, 1, 64, 1, F16, [40000, 33000]), (128, 2, 128, 1, BF16, [37000, 45000]), (128, 1, 256, 3, F16, [41000, 30000]),
+                                                           (64, 1, 128, 40, BF16, [90000, 61000])])
+def test_long_ranges(dev, heads, group, D, N, dtype, lengths):
+    """Few workgroups a head: ranges of hundreds of pages, cut inside a sequence."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(heads + D)
+    cache, M = filled(dev, lengths, heads, D, dtype)
+    q = torch.randn(2, heads * group, N, D, generator=g).to(dtype).to(dev)
+    some = [0, 1, heads * group // 2, heads * group - 2, heads * group - 1]
+    for mask in masks_of(g, dev, 2, heads * group, 1, M, lengths):
+        o, lse = fm.cache_attention_lse(q, cache, mask, scale_of(D))
+        agrees(o, lse, q, cache, [0, 1], some, mask, [N, N])
+    cache.check()
+
+
+@pytest.mark.parametrize("B,group,N,D,dtype", [(130, 4, 128, 64, F16), (150, 3, 150, 128, BF16), (1030, 3, 21, 256, F16)])
+def test_many_pieces_with_masks(dev, B, group, N, D, dtype):
+    """More tiles than ranges are made for, with the mask's rows of 64 queries, one of the sequences long."""
+    import fa2_custom_mask as fm
+    g = torch.Generator().manual_seed(B)
+    lengths = [1 + (61 * b) % 500 for b in range(B)]
+    lengths[5], lengths[B - 1] = 5000, 17000
+    counts = [min(n, N if b % 2 else 1 + b % N) for b, n in enumerate(lengths)]
+    assert B * -(-N * group // 32) > 2048
+    cache, M = filled(dev, lengths, 1, D, dtype)
+    q = torch.randn(B, group, N, D, generator=g).to(dtype).to(dev)
+    for mask in masks_of(g, dev, B, group, -(-N // PAGE), M, lengths):
+        o, lse = fm.cache_attention_lse(q, cache, mask, scale_of(D), counts=ints(counts, dev))
+        agrees(o, lse, q, cache, [0, 1, 5, 6, 77, B - 1], range(group), mask, counts)
+        assert not bool(o[0, :, counts[0]:].any())
+    cache.check()
+
+
 def test_large_scores(dev):
     """A maximum that grows from page to page, scores that 32 bits of an exponential cannot hold."""
     g = torch.Generator().manual_seed(12)
