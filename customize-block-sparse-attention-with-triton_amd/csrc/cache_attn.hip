@@ -750,12 +750,17 @@ static CachePlan cache_plan(const bsattn_cache& c, int B, int H, int N) {
   p.units = (int64_t)B * p.tiles;
   const int per_cu = p.qt == 1 ? (c.head_dim < 128 ? 3 : 2) : (p.qt == 2 && c.head_dim < 256 ? 2 : 1);
   const int64_t fill = (int64_t)compute_units() * per_cu;
-  // ranges where a workgroup a unit would leave compute units idle or wait for the longest sequence (the axis is counted in 32 bits).  Sequences
-  // of one length do better without sooner, by 5 to 8 %; those of different lengths lose by it: 16 prompts of 1 000 to 9 000 tokens, 300 queries, 9 rounds
-  // of units 411 us in ranges, 491 without; 24 of 200 to 4 000, 5 rounds 81 and 94.  One token of many sequences: 256 of 200 to 16 000, 4 rounds
-  // 190 and 222, the same at 6 rounds; every workgroup looks through the units of its head, 1 000 of which take 53 us where a workgroup each takes 37.
-  const bool pieces = p.tiles > 1;
-  const bool ranges = p.units * c.heads < (pieces ? 16 : 6) * fill && p.units <= (pieces ? 2048 : 512) && p.units * ((int64_t)c.max_pages + STEP + GAP) < 0x7fffffffLL;
+  // Ranges wherever the device can find them, up to 2048 units of a head: the host does not know the lengths, and a workgroup a unit takes as long as
+  // the longest one, 0.29 us a page (us in ranges and with a workgroup a unit): 513 sequences of one head, one of them of 200 000 tokens, 30 and 897;
+  // 400 of 8 heads, 200 to 2 000 tokens and one of 100 000, 107 and 607, without that one 89 and 91, all of 1 000 tokens 101 and 103; 30 prompts, 300
+  // queries, 400 to 9 000 tokens 604 and 653, all of 4 000 798 and 795, of 400 and one of 60 000 534 and 1 101.  Two kinds of calls are better off without:
+  // - many units of one token that have a few pages each, through which every workgroup looks: 513 of 200 to 2 000 tokens 24 and 22, 2 000 of 50 to 500
+  //   31 and 22, 700 of 50 to 100 11 and 7.  No more than 64 pages a sequence, which the cache's tables say, bound what a long one costs there.
+  // - so many heads that few ranges are left for each, and a part of the GPU idle: 192 heads of 30 sequences 159 and 143, 300 heads 296 and 221 (100 heads
+  //   74 and 79).  Of few units these are in ranges all the same (192 heads of 4 sequences 24 and 27).
+  const bool pieces = p.tiles > 1, many_heads = c.heads > fill / 4;
+  const bool ranges = p.units <= 2048 && p.units * ((int64_t)c.max_pages + STEP + GAP) < 0x7fffffffLL &&      // (the axis is counted in 32 bits)
+                      (many_heads ? p.units * c.heads < (pieces ? 16 : 6) * fill : pieces || p.units <= 512 || c.max_pages > 64);
   p.W = ranges ? (int)std::max<int64_t>(1, fill / c.heads) : 0;
   return p;
 }

@@ -566,9 +566,11 @@ def masks_of(g, dev, B, H, rows, M, lengths):
     return [None] + [m.to(dev) for m in (one, each, thin)]
 
 
-@pytest.mark.parametrize("B,heads,group,D,dtype,longest", [(513, 1, 1, 64, F16, [17000]), (520, 1, 5, 128, BF16, [17100, 36000]), (600, 2, 2, 256, F16, [16500])])
+@pytest.mark.parametrize("B,heads,group,D,dtype,longest", [(513, 1, 1, 64, F16, [17000]), (520, 1, 5, 128, BF16, [17100, 36000]), (600, 2, 2, 256, F16, [16500]),
+                                                           (1500, 1, 3, 128, F16, [100000]), (2048, 8, 1, 64, BF16, [9000]), (2060, 1, 1, 64, F16, [17000]),
+                                                           (2100, 1, 5, 128, BF16, [17100, 36000]), (24, 200, 1, 64, F16, [17000]), (24, 200, 2, 256, BF16, [16500])])
 def test_long_ones_among_many_sequences(dev, B, heads, group, D, dtype, longest):
-    """A workgroup for each sequence, a few of them long."""
+    """A few long sequences among hundreds (in ranges) and thousands, or of very many heads (a workgroup for each)."""
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(B)
     lengths = [1 + (37 * b) % 100 for b in range(B)]
