@@ -1161,6 +1161,60 @@ def test_captured_steps(dev):
             cache.check(), eager.check()
 
 
+def test_graphs_that_share_a_pool(dev):
+    """Graphs of one memory pool, whose workspaces may lie in the same place, replayed in any order, beside eager calls: bookkeeping and
+    attention with parts of many workgroups, in 16 bits and in fp32."""
+    import fa2_custom_mask as fm
+    H, D, S, M = 2, 64, 4, 160
+    g = torch.Generator().manual_seed(23)
+    pair = [make(dev, 700, H, D, S, M * PAGE, BF16)[0] for _ in range(2)]
+    k, v = tokens(S, H, 9000, D, BF16, g, dev)
+    for c in pair:
+        fm.cache_append(c, k, v, counts=ints([9000, 5000, 70, 0], dev))
+    k1, v1 = tokens(S, H, 1, D, BF16, g, dev)
+    q1, q3 = [torch.randn(S, 4 * H, n, D, generator=g).to(BF16).to(dev) for n in (1, 3)]
+    mask = (torch.rand(1, 4 * H, 1, M, generator=g) < 0.5).to(dev)
+    three = ints([0, 1, 2], dev)
+    last, kept, child = ints([3], dev), ints([4000], dev, torch.int64), ints([1], dev, torch.int64)
+
+    def step(c):
+        fm.cache_append(c, k1[:3], v1[:3], sequences=three)
+        return fm.cache_attention_lse(q1, c, None, 0.1, out_fp32=True) + (fm.cache_attention(q3, c, mask, 0.1),)
+
+    def branch(c):
+        fm.cache_free(c, last)
+        fm.cache_fork(c, child, last)
+        fm.cache_free(c, last, kept)
+        fm.cache_append(c, k1[:1], v1[:1], sequences=last)
+        fm.cache_compact(c)
+        return fm.cache_attention_lse(q3, c, None, 0.1) + fm.cache_read(c, 70, start=c.lengths - 60)
+
+    calls = (step, branch)
+    cache, eager = pair
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for q in (q1, q3):
+            fm.cache_attention_lse(q, cache, None, 0.1, out_fp32=True)
+            fm.cache_attention(q, cache, mask, 0.1)
+    torch.cuda.current_stream().wait_stream(stream)
+    graphs, outs = [], []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            outs.append(call(cache))
+    for i in (0, 1, 0, 0, 1, 1, 0):
+        for x in (k1, v1, q1, q3):
+            x.copy_(torch.randn(x.shape, generator=g).to(BF16))
+        graphs[i].replay()
+        want = calls[i](eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want)), i
+        assert torch.equal(cache.page_table, eager.page_table) and torch.equal(cache.lengths, eager.lengths) and torch.equal(cache.refs, eager.refs)
+        assert torch.equal(cache.free_from, eager.free_from)
+        cache.check(), eager.check()
+
+
 def test_threads(dev):
     """Two threads, each with a cache and a stream of its own, and two that share both kinds of calls on one stream."""
     import threading
