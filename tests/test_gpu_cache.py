@@ -801,18 +801,21 @@ def test_free_and_fork_by_the_cache_s_own_numbers(dev):
     """keep, sequences, parents and children that are the cache's tables themselves: they count as they were before the call."""
     import fa2_custom_mask as fm
     g = torch.Generator().manual_seed(18)
-    S = 2000
-    cache, ref = make(dev, 2 * S, 1, 64, S, 128, F16)
-    for _ in range(5):
-        first = [int(x) for x in torch.randint(1, 129, (1000,), generator=g)]
-        for rows in (list(range(1000)), list(range(1000, S))):
-            assert not append(cache, ref, *tokens(1000, 1, 128, 64, F16, g, dev), counts=first, sequences=rows)
-        order = torch.randperm(S, generator=g).tolist()
-        fm.cache_free(cache, ints(order, dev), keep=cache.lengths)            # sequence order[i] to the length of sequence i
-        assert not ref.free(order, list(ref.length))
-        same_tables(cache, ref)
-        fm.cache_free(cache)
-        ref.free()
+    S = 30000                                                               # (many times the workgroups that are on the GPU at once)
+    cache = fm.PagedCache4(2 * S, 1, 64, S, 128, F16, dev)
+    for _ in range(3):
+        lengths = torch.randint(1, 129, (S,), generator=g, dtype=torch.int32)
+        pages = torch.arange(2 * S, dtype=torch.int32).view(S, 2)
+        pages[lengths <= PAGE, 1] = -1
+        cache.page_table.copy_(pages), cache.lengths.copy_(lengths)
+        cache.refs.zero_()[pages[pages >= 0].long().to(dev)] = 1
+        order = torch.randperm(S, generator=g)
+        fm.cache_free(cache, order.to(dev), keep=cache.lengths)               # sequence order[i] to the length of sequence i
+        want = lengths.clone()
+        want[order] = torch.minimum(lengths[order], lengths)
+        pages[want <= PAGE, 1] = -1
+        assert torch.equal(cache.lengths.cpu(), want) and torch.equal(cache.page_table.cpu(), pages)
+        assert int(cache.refs.sum()) == int((pages >= 0).sum()) == int((cache.refs > 0).sum())
     # lengths that are numbers of sequences: parents 3, 4, 5, and their children 0, 1, 2
     cache, ref = make(dev, 20, 1, 64, 6, 128, F16)
     append(cache, ref, *tokens(6, 1, 5, 64, F16, g, dev), counts=[0, 0, 0, 3, 4, 5])
